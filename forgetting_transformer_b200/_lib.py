@@ -119,6 +119,25 @@ _SIGNATURES = {
                                     c_int64, _F, _F, c_int64, c_int64, c_int64, _F]),
     "fox_token_shift_bwd": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, _F, c_int64, c_int64,
                                     c_int64, _F, _F, c_int64, c_int64, c_int64, _F, _F, _F, _F]),
+    "fox_rotary": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, _T4P, _F, c_int64, c_int, c_float,
+                        c_int, _F, c_int, c_int64, c_int64, c_int64, _T4P]),
+    "fox_qk_norm_rotary_fwd": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, _T4P, _T4P, _F,
+                        c_int, c_int64, _F, c_int, c_int64, c_float, _F, c_int64, c_int, c_float, _F, c_int, c_int64,
+                        c_int64, c_int64, _T4P, _T4P]),
+    "fox_qk_norm_rotary_partials": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "fox_qk_norm_rotary_bwd": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, _T4P, _T4P, _F,
+                        c_int, c_int64, _F, c_int, c_int64, c_float, _F, c_int64, c_int, c_float, _F, c_int, c_int64,
+                        c_int64, c_int64, _T4P, _T4P, _T4P, _T4P, _F, _F, _F]),
+    "fox_page_tables": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, _F, _F, _F, c_int64, _F, c_int64, _F,
+                        _F, _F, _F, _F, _F, _F, _F, _F]),
+    "fox_release_pages": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, _F, _F, _F, c_int64, _F, c_int64, _F]),
+    "fox_paged_update": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _F, c_int64,
+                        c_int64, _F, c_int64, c_int64, c_int, _F, c_int64, c_int64, _T4P, _T4P, _F, c_int64, c_int64, _F,
+                        c_int]),
+    "fox_paged_attn_workspace_floats": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
+    "fox_paged_attn": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _F,
+                        c_int64, c_int64, _T4P, _T4P, _F, c_int64, c_int64, _F, c_int64, _F, c_float, _F, c_int64, c_int64,
+                        _F, _F]),
 }
 
 _lock = threading.Lock()

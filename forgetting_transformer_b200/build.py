@@ -30,9 +30,10 @@ def host_path(torch_version: str = torch.__version__) -> str:
 
 
 HOST_PATH = host_path()
-SOURCES = ["fox_scan.cu", "fox_attn_fwd.cu", "fox_attn_bwd.cu", "fox_attn_bwd_dq.cu", "fox_attn_bwd_kv.cu", "fox_decode.cu", "fox_normgate.cu", "fox_rmsnorm.cu", "fox_shift.cu", "fox_glu.cu", "fox_ce.cu", "fox_block.cu", "fox_step.cu", "fox_noalloc.cu"]
+SOURCES = ["fox_scan.cu", "fox_attn_fwd.cu", "fox_attn_bwd.cu", "fox_attn_bwd_dq.cu", "fox_attn_bwd_kv.cu", "fox_decode.cu", "fox_normgate.cu", "fox_rmsnorm.cu", "fox_shift.cu", "fox_glu.cu", "fox_ce.cu", "fox_block.cu", "fox_step.cu", "fox_noalloc.cu",
+           "fox_rotary.cu", "fox_paged.cu", "fox_paged_attn.cu"]
 HEADERS = ["fox_common.cuh", "fox_host.h", os.path.join("..", "..", "include", "fox_b200.h")]
-HOST_SOURCES = ["host_module.cpp", "host_attention.cpp", "host_block.cpp", "host_gemm.cpp"]
+HOST_SOURCES = ["host_module.cpp", "host_attention.cpp", "host_block.cpp", "host_gemm.cpp", "host_serving.cpp"]
 HOST_HEADERS = ["host_common.h", "host_attention.h", "host_block.h", "host_gemm.h", os.path.join("..", "..", "include", "fox_b200.h")]
 
 

@@ -86,7 +86,8 @@ inline bool tma_ready(const Tensor& x) {
     if (sz[i] != 1 && ((st[i] * es) % 16 || st[i] <= 0)) return false;
   return true;
 }
-inline Tensor tma_view(const Tensor& x) { return tma_ready(x) ? x : x.contiguous(); }
+// (a view may be contiguous and yet begin inside 16 bytes: a copy then has to be made all the same)
+inline Tensor tma_view(const Tensor& x) { return tma_ready(x) ? x : x.clone(at::MemoryFormat::Contiguous); }
 inline Tensor empty_like_tma(const Tensor& x) {
   Tensor o = at::empty_like(x);
   return tma_ready(o) ? o : at::empty(x.sizes(), x.options());
@@ -129,3 +130,12 @@ FOX_PY(py_attention_backward);
 FOX_PY(py_set_block_classes);
 FOX_PY(py_block);
 FOX_PY(py_block_step);
+FOX_PY(py_rotary);
+FOX_PY(py_rotary_apply);
+FOX_PY(py_qk_norm_rotary);
+FOX_PY(py_qk_norm_rotary_forward);
+FOX_PY(py_qk_norm_rotary_backward);
+FOX_PY(py_page_tables);
+FOX_PY(py_release_pages);
+FOX_PY(py_paged_update);
+FOX_PY(py_paged_attention);

@@ -177,6 +177,15 @@ static PyMethodDef g_methods[] = {
     FOX_METHOD("set_block_classes", py_set_block_classes),
     FOX_METHOD("block", py_block),
     FOX_METHOD("block_step", py_block_step),
+    FOX_METHOD("rotary", py_rotary),
+    FOX_METHOD("rotary_apply", py_rotary_apply),
+    FOX_METHOD("qk_norm_rotary", py_qk_norm_rotary),
+    FOX_METHOD("qk_norm_rotary_forward", py_qk_norm_rotary_forward),
+    FOX_METHOD("qk_norm_rotary_backward", py_qk_norm_rotary_backward),
+    FOX_METHOD("page_tables", py_page_tables),
+    FOX_METHOD("release_pages", py_release_pages),
+    FOX_METHOD("paged_update", py_paged_update),
+    FOX_METHOD("paged_attention", py_paged_attention),
     {nullptr, nullptr, 0, nullptr}};
 static PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_fox_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

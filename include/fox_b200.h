@@ -451,6 +451,69 @@ int fox_attn_bwd_noalloc(int device, void* stream, int dtype, int64_t B, int64_t
                          float* dlog_fgate, int32_t* status);
 int64_t fox_noalloc_scratch_floats(void);
 
+/* ---------------------------------------------------------------- rotary positions
+ * y = x with the pairs (i, i + half), interleaved: (2i, 2i + 1), i < half, of the first 2 half <= D channels turned by
+ * position * inv_freq[i] and scaled (rotary.py:22-153, there from a table); the angle's product and reduction in 64 bits.
+ * inverse: by the negative angle, which is the backward.  x, y: (B,H,T,D) 16-bit views as everywhere; positions: int32, or
+ * int64 with pos_64, element strides (pos_sb, pos_st), or NULL: first + t.  D in {16,32,64,128}; H <= 65535,
+ * B T <= 2^31 - 65536 (FOX_ERR_TOO_LARGE). */
+int fox_rotary(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t D, const fox_tensor4* x,
+               const float* inv_freq, int64_t half, int interleaved, float scale, int inverse, const void* positions, int pos_64,
+               int64_t pos_sb, int64_t pos_st, int64_t first, const fox_tensor4* y);
+
+/* The per-head RMSNorm of q (H heads) and k (Hk heads) and their rotation in one launch (layernorm.py:183-245, rotary.py:22-153;
+ * modeling_forgetting_transformer.py:264-265, 314-316).  wq, wk: (heads * D) with stride wq_sh = D, or one (D) for all heads with
+ * wq_sh = 0; w*_dtype any FOX_DTYPE_*. */
+int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
+                           const fox_tensor4* q, const fox_tensor4* k, const void* wq, int wq_dtype, int64_t wq_sh,
+                           const void* wk, int wk_dtype, int64_t wk_sh, float eps, const float* inv_freq, int64_t half,
+                           int interleaved, float scale, const void* positions, int pos_64, int64_t pos_sb, int64_t pos_st,
+                           int64_t first, const fox_tensor4* q_out, const fox_tensor4* k_out);
+/* Its backward, from the inputs and the gradients of the results (dq_out, dk_out): dq, dk, and dwq, dwk in the weights' types and
+ * shapes.  dw_partial: fox_qk_norm_rotary_partials(...) * (H + Hk) * D floats, 16-byte aligned, fully overwritten. */
+int64_t fox_qk_norm_rotary_partials(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D);
+int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
+                           const fox_tensor4* q, const fox_tensor4* k, const void* wq, int wq_dtype, int64_t wq_sh,
+                           const void* wk, int wk_dtype, int64_t wk_sh, float eps, const float* inv_freq, int64_t half,
+                           int interleaved, float scale, const void* positions, int pos_64, int64_t pos_sb, int64_t pos_st,
+                           int64_t first, const fox_tensor4* dq_out, const fox_tensor4* dk_out, const fox_tensor4* dq,
+                           const fox_tensor4* dk, float* dw_partial, void* dwq, void* dwk);
+
+/* ---------------------------------------------------------------- paged generation cache
+ * The counterpart of upstream's growing cache (fgate_cache.py:77-116) for requests of different lengths.  A pool of n_pages
+ * pages of `page` tokens (a power of two, 16 to 65536); token t of request r is row t % page of page
+ * block_table[r * table_ld + t / page], its slot is that page * page + the row.  Free pages are a stack, free_pages[0 .. num_free).
+ * All of these arrays are int32 on the device.
+ *
+ * Pages for new_tokens[r] more tokens of every request, in order: lengths_out = lengths + what was granted, the table's new
+ * entries, num_free_out, starts (R + 1) = the packed batch's first token of every request, granted (R) = new_tokens, or 0 for a
+ * request whose tokens find no room (its table row of `width` entries, max_tokens, the free pages), and for each of the packed
+ * batch's max_tokens places its request (-1: none), position (0) and slot (-1: none, or not granted).  lengths_out and
+ * num_free_out may be lengths and num_free.  workspace: R + 1. */
+int fox_page_tables(int device, void* stream, int64_t R, int64_t width, int64_t page, int64_t max_tokens, const int32_t* lengths,
+                    const int32_t* new_tokens, int32_t* block_table, int64_t table_ld, const int32_t* free_pages, int64_t n_pages,
+                    const int32_t* num_free, int32_t* lengths_out, int32_t* num_free_out, int32_t* starts, int32_t* granted,
+                    int32_t* requests, int32_t* positions, int32_t* slots, int32_t* workspace);
+/* Cuts every request to its first keep[r] tokens (longer than it is: as it is) and puts the pages behind them back on the stack, in place. */
+int fox_release_pages(int device, void* stream, int64_t R, int64_t width, int64_t page, int32_t* lengths, const int32_t* keep,
+                      int32_t* block_table, int64_t table_ld, int32_t* free_pages, int64_t n_pages, int32_t* num_free);
+/* Rows of T tokens into their slots (int32, or int64 with slots_64; one outside the pool: the token is left out).  k, v: (T, Hk, D)
+ * 16-bit; gates (T, H), gate_kind as in fox_attn_prologue.  k_pages, v_pages: (n_pages, Hk, page, D), strides sb of pages, sh of
+ * heads, st of rows; gate_pages (n_pages, H, page) fp32, strides gp_sp, gp_sh and 1. */
+int fox_paged_update(int device, void* stream, int64_t T, int64_t H, int64_t Hk, int64_t D, int64_t n_pages, int64_t page,
+                     const void* k, int64_t k_st, int64_t k_sh, const void* v, int64_t v_st, int64_t v_sh, int gate_kind,
+                     const void* gates, int64_t g_st, int64_t g_sh, const fox_tensor4* k_pages, const fox_tensor4* v_pages,
+                     float* gate_pages, int64_t gp_sp, int64_t gp_sh, const void* slots, int slots_64);
+/* Forward attention of one query row per request, q (R, H, D), against its lengths[r] keys (0: out 0, L -inf); query head h reads
+ * key head h / (H / Hk) and its own gates.  A table entry outside the pool leaves its keys out.  o (R, H, D); L (R, H) fp32 or
+ * NULL; gate strides multiples of 4; workspace: fox_paged_attn_workspace_floats(...), 16-byte aligned. */
+int64_t fox_paged_attn_workspace_floats(int64_t R, int64_t H, int64_t Hk, int64_t D);
+int fox_paged_attn(int device, void* stream, int dtype, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t n_pages, int64_t page,
+                   int64_t width, const void* q, int64_t q_sr, int64_t q_sh, const fox_tensor4* k_pages,
+                   const fox_tensor4* v_pages, const float* gate_pages, int64_t gp_sp, int64_t gp_sh, const int32_t* block_table,
+                   int64_t table_ld, const int32_t* lengths, float sm_scale, void* o, int64_t o_sr, int64_t o_sh, float* L,
+                   float* workspace);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,260 @@
+"""Rotary positions and the q / k norms with the rotation, against the formulas in 64 bits.
+
+Bounds.  The result is rounded once to 16 bits: half a step, eps / 2 of the value (fp16: and 2^-25 where it is subnormal).  In
+front of that the kernels work in fp32: the reduced angle, at most pi, is off by 2^-23 when it becomes fp32, sine and cosine by
+an ulp or two more, and a turned value adds two products: together below 2^-21 of |a| + |b| for the pair (a, b).  A norm's 1 / rms is off by half of its sum's
+error (8 + log2(D / 8) roundings of terms of one sign) and two ulp: below 2^-20 of its value, so that a normed pair gets 2^-19."""
+import itertools
+
+import pytest
+import torch
+
+import forgetting_transformer_b200 as fox
+
+pytestmark = pytest.mark.gpu
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def tiny(dtype):
+    return 2.0 ** -25 if dtype == torch.float16 else 0.0
+
+
+def pairs(half, interleaved, device):
+    i = torch.arange(half, device=device)
+    return (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+
+
+def turn64(x, angles, interleaved, scale=1.0, sign=1.0):
+    """x (..., D) in 64 bits; angles (..., half), broadcast over x's leading axes."""
+    a, b = pairs(angles.shape[-1], interleaved, x.device)
+    c, s = scale * angles.cos(), scale * sign * angles.sin()
+    y = x.clone()
+    y[..., a] = x[..., a] * c - x[..., b] * s
+    y[..., b] = x[..., b] * c + x[..., a] * s
+    return y
+
+
+def reach(x, half, interleaved, scale=1.0):
+    """|a| + |b| of the pair that each channel belongs to, |x| where it belongs to none."""
+    a, b = pairs(half, interleaved, x.device)
+    m = x.abs().clone()
+    m[..., a] = m[..., b] = (x[..., a].abs() + x[..., b].abs()) * max(scale, 1.0)
+    return m
+
+
+def norm64(x, w, eps):
+    return x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps) * w
+
+
+def angles64(positions, inv_freq):
+    return positions.double()[..., None] * inv_freq.double()
+
+
+def data(seed, *shape, dtype):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+SHAPES = [(1, 1, 1, 16, 16), (2, 17, 3, 32, 32), (1, 130, 24, 64, 64), (3, 33, 5, 64, 32), (2, 65, 7, 128, 128), (1, 40, 33, 128, 20),
+          (2, 19, 4, 64, 2), (1, 700, 9, 16, 10), (1, 9, 260, 16, 8)]
+
+
+@pytest.mark.parametrize("B,T,H,D,rot", SHAPES)
+@pytest.mark.parametrize("interleaved,head_first", list(itertools.product([False, True], [False, True])))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rotary_and_its_gradient(B, T, H, D, rot, interleaved, head_first, dtype):
+    scale = 1.25
+    x = data(B * T + D, B, T, H, D, dtype=dtype)
+    dy = data(B * T + D + 1, B, T, H, D, dtype=dtype)
+    inv_freq, _ = fox.rotary_frequencies(rot, device="cuda")
+    pos = torch.randint(0, 5000, (B, T), generator=torch.Generator().manual_seed(T)).cuda()
+    lay = (lambda t: t.transpose(1, 2)) if head_first else (lambda t: t)
+    xin = lay(x).detach().requires_grad_()
+    y = fox.rotary_embedding(xin, inv_freq, pos, head_first=head_first, interleaved=interleaved, scale=scale)
+    assert y.dtype == dtype and y.shape == xin.shape
+    (dx,) = torch.autograd.grad(y, xin, lay(dy))
+    a = angles64(pos, inv_freq)[:, :, None]
+    for got, src, sign in ((y, x, 1.0), (dx, dy, -1.0)):
+        ref = turn64(src.double(), a, interleaved, scale, sign)
+        tol = half_step(dtype) * ref.abs() + 2 ** -21 * reach(src.double(), rot // 2, interleaved, scale) + tiny(dtype)
+        err = (lay(got).double() - ref).abs()
+        assert (err <= tol).all(), (err - tol).max().item()
+
+
+@pytest.mark.parametrize("where", ["none", "int", "int32", "strided"])
+def test_positions_in_every_form(where):
+    x = data(3, 2, 50, 3, 64, dtype=torch.bfloat16)
+    inv_freq, _ = fox.rotary_frequencies(64, device="cuda")
+    given, at = {"none": (None, torch.arange(50)), "int": (1234567, 1234567 + torch.arange(50)),
+                 "int32": (torch.arange(7, 57, dtype=torch.int32).cuda(), torch.arange(7, 57)),
+                 "strided": (torch.arange(100, device="cuda")[::2], torch.arange(0, 100, 2))}[where]
+    y = fox.rotary_embedding(x, inv_freq, given)
+    ref = turn64(x.double(), angles64(at.cuda(), inv_freq)[:, None], False)
+    tol = 2 ** -8 * ref.abs() + 2 ** -21 * reach(x.double(), 32, False)
+    assert ((y.double() - ref).abs() <= tol).all()
+    one = fox.rotary_embedding(x[1], inv_freq, given)       # a packed batch: three dimensions
+    assert torch.equal(one, y[1])
+
+
+@pytest.mark.parametrize("first", [-70000, 2 ** 20 + 1, 2 ** 31 - 40, 2 ** 40])
+def test_angles_of_far_positions(first):
+    """The product of position and frequency in 64 bits: its own rounding is 2^-53 of up to 2^40 radians, far below 2^-21 up to
+    2^31; at 2^40 it is 2^-13 at the fastest frequency, which both sides share."""
+    x = data(5, 1, 30, 2, 64, dtype=torch.float16)
+    inv_freq, _ = fox.rotary_frequencies(64, device="cuda")
+    y = fox.rotary_embedding(x, inv_freq, first)
+    ref = turn64(x.double(), angles64(first + torch.arange(30, device="cuda"), inv_freq)[:, None], False)
+    tol = 2 ** -11 * ref.abs() + 2 ** -21 * reach(x.double(), 32, False) + 2 ** -25
+    assert ((y.double() - ref).abs() <= tol).all()
+
+
+def test_strided_views_and_empty():
+    """Slices of a projection's row, an expanded batch, a view that 16-byte loads cannot take, and no tokens."""
+    inv_freq, _ = fox.rotary_frequencies(32, device="cuda")
+    big = data(8, 2, 21, 9 * 64 + 3, dtype=torch.bfloat16)
+    for x in (big[:, :, 64:4 * 64].view(2, 21, 3, 64), big[:, :, 3:3 + 3 * 64].view(2, 21, 3, 64),
+              big[:1, :, :192].view(1, 21, 3, 64).expand(4, -1, -1, -1), big[:, ::2, :128].view(2, 11, 2, 64)):
+        y = fox.rotary_embedding(x, inv_freq)
+        assert torch.equal(y, fox.rotary_embedding(x.contiguous(), inv_freq))
+    empty = big[:, :0, :128].view(2, 0, 2, 64).detach().requires_grad_()
+    y = fox.rotary_embedding(empty, inv_freq)
+    assert y.shape == empty.shape
+    (dx,) = torch.autograd.grad(y, empty, torch.zeros_like(y))
+    assert dx.shape == empty.shape
+
+
+NORMS = [(1, 1, 1, 1, 16, 16), (2, 37, 4, 2, 32, 32), (1, 130, 24, 24, 64, 64), (2, 70, 6, 3, 64, 40), (1, 300, 16, 16, 128, 128),
+         (3, 11, 33, 11, 128, 64), (1, 2100, 5, 5, 64, 12), (1, 5, 140, 70, 16, 4)]
+
+
+@pytest.mark.parametrize("B,T,H,Hk,D,rot", NORMS)
+@pytest.mark.parametrize("interleaved,shared", list(itertools.product([False, True], [False, True])))
+@pytest.mark.parametrize("dtype,w_dtype", [(torch.bfloat16, torch.float32), (torch.float16, torch.float16),
+                                           (torch.bfloat16, torch.bfloat16)])
+def test_norm_rotary_and_its_gradients(B, T, H, Hk, D, rot, interleaved, shared, dtype, w_dtype):
+    eps, scale = 1e-5, 1.1
+    inv_freq, _ = fox.rotary_frequencies(rot, device="cuda")
+    x = [data(T + i, B, T, h, D, dtype=dtype) for i, h in enumerate((H, Hk))]
+    w = [(1 + 0.3 * data(T + 2 + i, D if shared else h * D, dtype=torch.float32)).to(w_dtype) for i, h in enumerate((H, Hk))]
+    dy = [data(T + 4 + i, B, T, h, D, dtype=dtype) for i, h in enumerate((H, Hk))]
+    leaves = [t.detach().requires_grad_() for t in (*x, *w)]
+    out = fox.qk_norm_rotary(*leaves, inv_freq, 77, eps=eps, interleaved=interleaved, scale=scale)
+    grads = torch.autograd.grad(out, leaves, dy)
+    a = angles64(77 + torch.arange(T, device="cuda"), inv_freq)[:, None]
+    parts = 600                                     # (at most: shares of the weights' gradients, 148 * 4)
+    h16 = half_step(dtype)
+    for i in range(2):
+        x64, w64 = x[i].double(), w[i].double().view(-1, D)
+        n = norm64(x64, w64, eps)
+        ref = turn64(n, a, interleaved, scale)
+        tol = h16 * ref.abs() + 2 ** -19 * reach(n, rot // 2, interleaved, scale) + tiny(dtype)
+        assert ((out[i].double() - ref).abs() <= tol).all()
+        dn = turn64(dy[i].double(), a, interleaved, scale, -1.0)
+        m = reach(dy[i].double(), rot // 2, interleaved, scale)          # what dn's error is measured by
+        r = torch.rsqrt(x64.pow(2).mean(-1, keepdim=True) + eps)
+        xhat = x64 * r
+        dx = r * (dn * w64 - xhat * (dn * w64 * xhat).mean(-1, keepdim=True))
+        size = r * (m * w64.abs() + xhat.abs() * (m * w64 * xhat).abs().mean(-1, keepdim=True))
+        assert grads[i].dtype == dtype
+        # (dn 2^-21, r twice 2^-20, the products and the mean's sum of D terms 2^-20: below 2^-18 of the terms' sizes)
+        assert ((grads[i].double() - dx).abs() <= h16 * dx.abs() + 2 ** -18 * size + tiny(dtype)).all()
+        axes = (0, 1, 2) if shared else (0, 1)
+        heads = (H, Hk)[i]
+        dw = (dn * xhat).sum(axes).flatten()
+        terms = (m * xhat.abs()).sum(axes).flatten()
+        chain = B * T + 16 if B * T < parts else B * T / 148 + 16        # of a thread, of the shares, of the last sums
+        chain += parts / 16 * (heads if shared else 1) + 16
+        tol = (2 ** -19 + chain * 2 ** -24) * terms
+        if w_dtype != torch.float32:
+            tol = tol + half_step(w_dtype) * dw.abs() + tiny(w_dtype)
+        assert grads[2 + i].dtype == w_dtype and grads[2 + i].shape == w[i].shape
+        assert ((grads[2 + i].double() - dw).abs() <= tol).all()
+
+
+def test_norm_rotary_gradient_against_differences():
+    """The gradients' products with a direction against central differences of the 64-bit formula.  The differences' own error
+    is of third order (step 1e-4: below 1e-7 of the sum of sizes); the gradients' is their rounding, bounded as above."""
+    B, T, H, Hk, D = 1, 24, 4, 2, 64
+    inv_freq, _ = fox.rotary_frequencies(48, device="cuda")
+    x = [data(i, B, T, h, D, dtype=torch.float16) for i, h in enumerate((H, Hk))]
+    w = [1 + 0.2 * data(2 + i, h * D, dtype=torch.float32) for i, h in enumerate((H, Hk))]
+    dy = [data(4 + i, B, T, h, D, dtype=torch.float16) for i, h in enumerate((H, Hk))]
+    leaves = [t.detach().requires_grad_() for t in (*x, *w)]
+    out = fox.qk_norm_rotary(*leaves, inv_freq, None)
+    grads = torch.autograd.grad(out, leaves, dy)
+    a = angles64(torch.arange(T, device="cuda"), inv_freq)[:, None]
+    f = lambda i, xx, ww: (turn64(norm64(xx, ww.view(-1, D), 1e-5), a, False) * dy[i].double()).sum()
+    for i in range(2):
+        for k, (base, grad) in enumerate(((x[i].double(), grads[i]), (w[i].double(), grads[2 + i]))):
+            d = data(9 + i, *base.shape, dtype=torch.float32).double()
+            args = lambda t: (t, w[i].double()) if k == 0 else (x[i].double(), t)
+            diff = (f(i, *args(base + 1e-4 * d)) - f(i, *args(base - 1e-4 * d))) / 2e-4
+            off = (2 ** -11 if k == 0 else 2 ** -17) * (grad.double().abs() * d.abs()).sum() + 2 ** -16 * d.abs().sum()
+            assert ((grad.double() * d).sum() - diff).abs() <= off
+
+
+def test_one_result_unused_and_frozen_inputs():
+    inv_freq, _ = fox.rotary_frequencies(64, device="cuda")
+    q, k = [data(i, 2, 9, 3, 64, dtype=torch.bfloat16).requires_grad_() for i in range(2)]
+    w = torch.ones(64, device="cuda")
+    out = fox.qk_norm_rotary(q, k, w, w, inv_freq)
+    dq, dk = torch.autograd.grad(out[0].float().sum(), [q, k], retain_graph=True)
+    assert dk.abs().max() == 0 and dq.abs().max() > 0
+    with torch.no_grad():
+        assert not fox.qk_norm_rotary(q, k, w, w, inv_freq)[0].requires_grad
+    frozen = fox.qk_norm_rotary(q.detach(), k, w, w, inv_freq)
+    (dk2,) = torch.autograd.grad(frozen[1].float().sum(), [k])
+    assert dk2.abs().max() > 0
+    torch.autograd.grad(out[1].float().sum(), [k])
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out[1].float().sum(), [k])
+
+
+def test_streams_and_graphs():
+    """On a stream of the caller's, forward and backward captured in a graph and replayed on new values."""
+    inv_freq, _ = fox.rotary_frequencies(64, device="cuda")
+    q, k = [data(i, 1, 40, 4, 64, dtype=torch.bfloat16).requires_grad_() for i in range(2)]
+    w = [torch.ones(256, device="cuda").requires_grad_() for _ in range(2)]
+    pos = torch.zeros(40, dtype=torch.int32, device="cuda")
+    dy = [data(5 + i, 1, 40, 4, 64, dtype=torch.bfloat16) for i in range(2)]
+
+    def step():
+        out = fox.qk_norm_rotary(q, k, *w, inv_freq, pos)
+        return [*out, *torch.autograd.grad(out, [q, k, *w], dy)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            got = step()
+        with torch.no_grad():
+            q.copy_(data(11, 1, 40, 4, 64, dtype=torch.bfloat16))
+            pos.copy_(torch.arange(100, 140))
+        g.replay()
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("scaling", [dict(scaling="linear", factor=4.0), dict(scaling="ntk", factor=4.0),
+                                     dict(scaling="yarn", factor=8.0, original_length=2048)])
+def test_rotary_module(scaling):
+    """The module's two ways, in a layer's type, with scaled frequencies; norms in front."""
+    m = fox.RotaryEmbedding(64, 500000.0, **scaling).cuda().bfloat16()
+    q, k = [data(i, 1, 30, 2, 64, dtype=torch.bfloat16) for i in range(2)]
+    f, s = fox.rotary_frequencies(64, 500000.0, **scaling)
+    assert f.dtype == torch.float32 and m.scale == s
+    a = angles64(5000 + torch.arange(30, device="cuda"), f.cuda())[:, None]
+    for got, x in zip(m(q, k, 5000), (q, k)):
+        ref = turn64(x.double(), a, False, s)
+        assert ((got.double() - ref).abs() <= 2 ** -8 * ref.abs() + 2 ** -21 * reach(x.double(), 32, False, s)).all()
+    w = torch.full((64,), 0.5, device="cuda")
+    for got, x in zip(m.norm(q, k, w, w, 5000), (q, k)):
+        n = norm64(x.double(), 0.5, 1e-5)
+        ref = turn64(n, a, False, s)
+        assert ((got.double() - ref).abs() <= 2 ** -8 * ref.abs() + 2 ** -19 * reach(n, 32, False, s)).all()

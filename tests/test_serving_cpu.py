@@ -1,0 +1,154 @@
+"""Refusals of the rotary and paged-cache operators, which come before anything runs on a GPU, and the frequencies."""
+import math
+
+import pytest
+import torch
+
+import forgetting_transformer_b200 as fox
+from forgetting_transformer_b200 import _lib
+
+
+def bf(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+F32 = torch.ones(32)
+
+
+@pytest.mark.parametrize("call,why", [
+    (lambda: fox.rotary_embedding(torch.zeros(1, 4, 2, 64), F32), "Only torch.float16"),
+    (lambda: fox.rotary_embedding(bf(4, 64), F32), "3 or 4 dimensions"),
+    (lambda: fox.rotary_embedding(bf(1, 4, 2, 48), F32), "head dims"),
+    (lambda: fox.rotary_embedding(bf(1, 4, 2, 32), F32), "inv_freq must have"),
+    (lambda: fox.rotary_embedding(bf(1, 4, 2, 64), F32[:0]), "inv_freq must have"),
+    (lambda: fox.rotary_embedding(bf(1, 4, 2, 64), F32.double()), "torch.float32"),
+    (lambda: fox.rotary_embedding(bf(1, 4, 2, 64), F32, torch.zeros(5, dtype=torch.int32)), "positions must have the shape"),
+    (lambda: fox.rotary_embedding(bf(2, 4, 2, 64), F32, torch.zeros(3, 4, dtype=torch.int32)), "positions must have the shape"),
+    (lambda: fox.rotary_embedding(bf(1, 4, 2, 64), F32, torch.zeros(4)), "torch.int32 or torch.int64"),
+    (lambda: fox.rotary_embedding(bf(1, 4, 2, 64), F32, 1.5), "integer"),
+    (lambda: fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 5, 2, 64), F32, F32, F32), "agree"),
+    (lambda: fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 2, 64).half(), F32, F32, F32), "agree"),
+    (lambda: fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 2, 64), torch.ones(32), torch.ones(64), F32), "q_weight"),
+    (lambda: fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 2, 64), torch.ones(64), torch.ones(64).int(), F32), "k_weight"),
+])
+def test_rotary_refusals(call, why):
+    with pytest.raises(AssertionError, match=why):
+        call()
+
+
+def test_no_cpu_path():
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    with pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.rotary_embedding(bf(1, 4, 2, 64), F32)
+    with pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 2, 64), torch.ones(64), torch.ones(128), F32)
+    with pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.page_tables(i(2), i(2), i(2, 3), i(5), i(1), 16, 4)
+    with pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.release_pages(i(2), i(2), i(2, 3), i(5), i(1), 16)
+    pool = pages()
+    with pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.paged_update(*pool, bf(4, 2, 64), bf(4, 2, 64), torch.zeros(4, 2), i(4))
+    with pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.paged_forgetting_attention(bf(3, 2, 64), *pool, i(3, 4), i(3))
+
+
+def pages(P=5, Hk=2, H=2, page=16, D=64, dtype=torch.bfloat16):
+    return (torch.zeros(P, Hk, page, D, dtype=dtype), torch.zeros(P, Hk, page, D, dtype=dtype), torch.zeros(P, H, page))
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(page=24), "power of two"), (dict(page=8), "power of two"), (dict(D=48), "head dims"), (dict(H=3), "multiple"),
+    (dict(dtype=torch.float32), "float16"),
+])
+def test_pool_refusals(change, why):
+    kw = dict(P=5, Hk=2, H=2, page=16, D=64, dtype=torch.bfloat16, **{})
+    kw.update(change)
+    with pytest.raises(AssertionError, match=why):
+        fox.paged_forgetting_attention(bf(3, kw["H"], kw["D"]), *pages(**kw), torch.zeros(3, 4, dtype=torch.int32),
+                                       torch.zeros(3, dtype=torch.int32))
+
+
+def test_paged_refusals():
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    k, v, g = pages()
+    att = fox.paged_forgetting_attention
+    for args, why in [((bf(3, 2, 32), k, v, g, i(3, 4), i(3)), "head dim"), ((bf(3, 1, 64), k, v, g, i(3, 4), i(3)), "heads"),
+                      ((bf(3, 2, 64).half(), k, v, g, i(3, 4), i(3)), "type"), ((bf(3, 2, 64), k, v, g, i(2, 4), i(3)), "request"),
+                      ((bf(3, 2, 64), k, v, g, i(3, 4).long(), i(3)), "int32"), ((bf(3, 2, 64), k, v, g, i(4, 3).t(), i(3)), "contiguous"),
+                      ((bf(3, 2, 64), k, v[:4], g, i(3, 4), i(3)), "equal shapes"), ((bf(3, 2, 64), k, v, g[:4], i(3, 4), i(3)), "gate_pages"),
+                      ((bf(3, 2, 64), k, v, g.double(), i(3, 4), i(3)), "float32"),
+                      ((bf(3, 2, 64), k, v, torch.zeros(5, 2, 17)[:, :, 1:], i(3, 4), i(3)), "16 bytes"),
+                      ((bf(3, 2, 64), torch.zeros(5, 2, 16, 68, dtype=torch.bfloat16)[..., 4:], v, g, i(3, 4), i(3)), "16 bytes"),
+                      ((bf(3, 2, 64), k.transpose(2, 3).contiguous().transpose(2, 3), v, g, i(3, 4), i(3)), "contiguous")]:
+        with pytest.raises(AssertionError, match=why):
+            att(*args)
+    with pytest.raises(_lib.FoxError, match="no gradients"):
+        att(bf(3, 2, 64).requires_grad_(), k, v, g, i(3, 4), i(3))
+    up = fox.paged_update
+    for args, why in [((k, v, g, bf(4, 3, 64), bf(4, 3, 64), torch.zeros(4, 2), i(4)), "heads"),
+                      ((k, v, g, bf(4, 2, 64), bf(3, 2, 64), torch.zeros(4, 2), i(4)), "heads"),
+                      ((k, v, g, bf(4, 2, 64).half(), bf(4, 2, 64), torch.zeros(4, 2), i(4)), "type"),
+                      ((k, v, g, bf(4, 2, 64), bf(4, 2, 64), torch.zeros(4, 3), i(4)), "gates"),
+                      ((k, v, g, bf(4, 2, 64), bf(4, 2, 64), bf(4, 2), i(4)), "float32"),
+                      ((k, v, g, bf(4, 2, 64), bf(4, 2, 64), torch.zeros(4, 2), i(5)), "slots"),
+                      ((k, v, g, bf(4, 2, 64), bf(4, 2, 64), torch.zeros(4, 2), torch.zeros(4)), "slots")]:
+        with pytest.raises(AssertionError, match=why):
+            up(*args)
+    with pytest.raises(_lib.FoxError, match="no gradients"):
+        up(k, v, g, bf(4, 2, 64).requires_grad_(), bf(4, 2, 64), torch.zeros(4, 2), i(4))
+    tab = fox.page_tables
+    for args, why in [((i(2), i(3), i(2, 3), i(5), i(1), 16, 4), "each request"), ((i(2), i(2), i(2, 3), i(5), i(2), 16, 4), "num_free"),
+                      ((i(2).long(), i(2), i(2, 3), i(5), i(1), 16, 4), "int32"), ((i(2), i(2), i(2, 3), i(5), i(1), 20, 4), "power of two"),
+                      ((i(2), i(2), i(2, 3), i(5), i(1), 16, -1), "max_tokens"), ((i(0), i(0), i(0, 3), i(5), i(1), 16, 4), "one at least"),
+                      ((i(2), i(2), i(1, 3).expand(2, 3), i(5), i(1), 16, 4), "overlap")]:
+        with pytest.raises(AssertionError, match=why):
+            tab(*args)
+    with pytest.raises(AssertionError, match="keep"):
+        fox.release_pages(i(2), i(3), i(2, 3), i(5), i(1), 16)
+
+
+def test_cache_refusals():
+    ok = dict(num_layers=1, num_pages=4, page_size=16, num_heads=4, head_dim=64, max_requests=2, max_length=40, device="cpu")
+    c = fox.PagedFgateCache(**ok)
+    assert c.block_table.shape == (2, 3) and c.free_pages.tolist() == [3, 2, 1, 0] and c.num_free.tolist() == [4] and len(c) == 1
+    for bad in (dict(page_size=24), dict(num_kv_heads=3), dict(num_pages=0), dict(max_length=0)):
+        with pytest.raises(ValueError):
+            fox.PagedFgateCache(**{**ok, **bad})
+
+
+def test_c_interface_refuses_sizes():
+    """Bad sizes come back as codes, before any device is touched (there is none here)."""
+    lib = _lib.load()
+    t, a = _lib.Tensor4(16, 8, 8, 8), 16
+    rot = lambda **c: lib.fox_rotary(*{**dict(dev=0, st=None, dt=1, B=1, T=1, H=1, D=64, x=t, f=a, half=32, inter=0, scale=1.0, inv=0, pos=None,
+                                             p64=0, sb=0, stt=0, first=0, y=t), **c}.values())
+    assert rot(D=48) == -2 and rot(half=33) == -1 and rot(half=0) == -1 and rot(B=0) == -1 and rot(dt=2) == -1
+    assert rot(T=2 ** 31) == -8 and rot(B=2 ** 20, T=2 ** 12) == -8 and rot(x=_lib.Tensor4(8, 8, 8, 8)) == -3 and rot(f=None) == -1
+    att = lambda **c: lib.fox_paged_attn(*{**dict(dev=0, st=None, dt=1, R=1, H=4, Hk=2, D=64, P=4, page=16, w=2, q=a, qr=8, qh=8, k=t, v=t, g=a, gp=4,
+                                                 gh=4, tab=a, ld=2, len=a, sc=1.0, o=a, orr=8, oh=8, L=None, ws=a), **c}.values())
+    assert att(D=8) == -2 and att(H=3) == -1 and att(page=17) == -1 and att(ld=1) == -1 and att(P=2 ** 28) == -8 and att(gp=2) == -3
+    assert att(R=0) == -1 and att(q=8) == -3 and att(ws=None) == -1
+    assert lib.fox_paged_attn_workspace_floats(0, 1, 1, 64) == 1 and lib.fox_qk_norm_rotary_partials(0, 0, 0, 0, 0) == 1
+
+
+def test_frequencies():
+    f, s = fox.rotary_frequencies(64)
+    assert s == 1.0 and f.dtype == torch.float32 and f.shape == (32,)
+    want = torch.tensor([10000.0 ** (-2 * i / 64) for i in range(32)], dtype=torch.float64)
+    assert ((f.double() - want).abs() <= 2 ** -24 * want).all()
+    lin, _ = fox.rotary_frequencies(64, scaling="linear", factor=4.0)
+    assert ((lin.double() * 4 - want).abs() <= 2 ** -24 * want).all()
+    ntk, _ = fox.rotary_frequencies(64, scaling="ntk", factor=4.0)
+    assert ntk[0] == 1 and abs(float(ntk[-1]) * 4 / float(want[-1]) - 1) < 2 ** -22
+    yarn, s = fox.rotary_frequencies(64, scaling="yarn", factor=8.0, original_length=4096)
+    assert s == pytest.approx(0.1 * math.log(8) + 1)
+    turns = 4096 * want / (2 * math.pi)
+    assert torch.equal(yarn[turns > 32], f[turns > 32])
+    slow = turns < 1
+    assert slow.any() and ((yarn[slow].double() * 8 - want[slow]).abs() <= 2 ** -24 * want[slow]).all()
+    assert (yarn[:-1] > yarn[1:]).all()
+    for bad in (dict(dim=63), dict(dim=0), dict(dim=64, scaling="yarn", factor=2.0), dict(dim=64, scaling="other"),
+                dict(dim=64, factor=0.0), dict(dim=2, scaling="ntk", factor=2.0)):
+        with pytest.raises(ValueError):
+            fox.rotary_frequencies(**bad)
