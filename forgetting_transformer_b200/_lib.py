@@ -137,7 +137,7 @@ _SIGNATURES = {
     "fox_paged_attn_workspace_floats": (c_int64, [c_int64, c_int64, c_int64, c_int64]),
     "fox_paged_attn": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _F,
                         c_int64, c_int64, _T4P, _T4P, _F, c_int64, c_int64, _F, c_int64, _F, c_float, _F, c_int64, c_int64,
-                        _F, _F]),
+                        _F, _F, _F]),
 }
 
 _lock = threading.Lock()

@@ -300,7 +300,7 @@ Pool check_pool(const Tensor& k, const Tensor& v, const Tensor& gates, int64_t g
   check_that(p.Hk >= 1 && p.H >= 1 && p.H % p.Hk == 0, "the heads of gate_pages must be a multiple of those of k_pages");
   for (const Tensor* t : {&k, &v}) {
     bool ok = t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0;
-    for (int i = 0; i < 3; ++i) ok = ok && (t->size(i) == 1 || t->stride(i) % 8 == 0);
+    for (int i = 0; i < 3; ++i) ok = ok && (t->size(i) == 1 || (t->stride(i) % 8 == 0 && t->stride(i) > 0));
     check_that(ok, "rows of k_pages and v_pages must be contiguous and start at multiples of 16 bytes");
   }
   bool ok = gates.stride(2) == 1 && reinterpret_cast<uintptr_t>(gates.data_ptr()) % (4 * gate_unit) == 0;
@@ -619,12 +619,13 @@ FOX_PY(py_paged_attention) {
       const fox_tensor4 kt = pages_t4(kp), vt = pages_t4(vp);
       const double sm_scale = args[6] == Py_None ? 1. / std::sqrt(static_cast<double>(p.D)) : given;
       auto g_stride = [&](int i) { return gp.size(i) == 1 ? p.page : gp.stride(i); };
+      int32_t* status = status_words(dev);
       launch("fox_paged_attn", st, [&] {
         return fox_paged_attn(dev, st, dtype_code(q.scalar_type()), R, p.H, p.Hk, p.D, p.P, p.page, table.size(1), q.data_ptr(),
                               axis_stride(q, 0), axis_stride(q, 1), &kt, &vt, gp.const_data_ptr<float>(), g_stride(0), g_stride(1),
                               table.const_data_ptr<int32_t>(), table_ld(table), lengths.const_data_ptr<int32_t>(),
                               static_cast<float>(sm_scale), o.data_ptr(), axis_stride(o, 0), axis_stride(o, 1),
-                              want_L ? L.mutable_data_ptr<float>() : nullptr, work.mutable_data_ptr<float>());
+                              want_L ? L.mutable_data_ptr<float>() : nullptr, work.mutable_data_ptr<float>(), status);
       });
     }
   }

@@ -506,13 +506,14 @@ int fox_paged_update(int device, void* stream, int64_t T, int64_t H, int64_t Hk,
                      float* gate_pages, int64_t gp_sp, int64_t gp_sh, const void* slots, int slots_64);
 /* Forward attention of one query row per request, q (R, H, D), against its lengths[r] keys (0: out 0, L -inf); query head h reads
  * key head h / (H / Hk) and its own gates.  A table entry outside the pool leaves its keys out.  o (R, H, D); L (R, H) fp32 or
- * NULL; gate strides multiples of 4; workspace: fox_paged_attn_workspace_floats(...), 16-byte aligned. */
+ * NULL; gate strides multiples of 4; workspace: fox_paged_attn_workspace_floats(...), 16-byte aligned;
+ * status as for fox_attn_fwd. */
 int64_t fox_paged_attn_workspace_floats(int64_t R, int64_t H, int64_t Hk, int64_t D);
 int fox_paged_attn(int device, void* stream, int dtype, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t n_pages, int64_t page,
                    int64_t width, const void* q, int64_t q_sr, int64_t q_sh, const fox_tensor4* k_pages,
                    const fox_tensor4* v_pages, const float* gate_pages, int64_t gp_sp, int64_t gp_sh, const int32_t* block_table,
                    int64_t table_ld, const int32_t* lengths, float sm_scale, void* o, int64_t o_sr, int64_t o_sh, float* L,
-                   float* workspace);
+                   float* workspace, int32_t* status);
 
 #ifdef __cplusplus
 }

@@ -126,9 +126,9 @@ def test_c_interface_refuses_sizes():
     assert rot(D=48) == -2 and rot(half=33) == -1 and rot(half=0) == -1 and rot(B=0) == -1 and rot(dt=2) == -1
     assert rot(T=2 ** 31) == -8 and rot(B=2 ** 20, T=2 ** 12) == -8 and rot(x=_lib.Tensor4(8, 8, 8, 8)) == -3 and rot(f=None) == -1
     att = lambda **c: lib.fox_paged_attn(*{**dict(dev=0, st=None, dt=1, R=1, H=4, Hk=2, D=64, P=4, page=16, w=2, q=a, qr=8, qh=8, k=t, v=t, g=a, gp=4,
-                                                 gh=4, tab=a, ld=2, len=a, sc=1.0, o=a, orr=8, oh=8, L=None, ws=a), **c}.values())
+                                                 gh=4, tab=a, ld=2, len=a, sc=1.0, o=a, orr=8, oh=8, L=None, ws=a, status=a), **c}.values())
     assert att(D=8) == -2 and att(H=3) == -1 and att(page=17) == -1 and att(ld=1) == -1 and att(P=2 ** 28) == -8 and att(gp=2) == -3
-    assert att(R=0) == -1 and att(q=8) == -3 and att(ws=None) == -1
+    assert att(R=0) == -1 and att(q=8) == -3 and att(ws=None) == -1 and att(status=None) == -1
     assert lib.fox_paged_attn_workspace_floats(0, 1, 1, 64) == 1 and lib.fox_qk_norm_rotary_partials(0, 0, 0, 0, 0) == 1
 
 
