@@ -6,8 +6,9 @@
 // Bound by reading every key, value and gate once.
 //
 // Work is counted in tiles of 16 keys of one unit (a request and a key head, with up to 8 of the query heads that share it).
-// All tiles of all units stand in one row, which is cut into equal ranges, one for each warp of a grid that fills the GPU
-// once: the longest request and the shortest cost what their tiles cost.  Every warp sums up the lengths by itself (its CTA
+// All tiles of all units stand in one row, with kPagStart places more in front of each unit for what its start costs; the row is
+// cut into equal ranges, one for each warp of a grid that fills the GPU once: the longest request and the shortest cost what
+// their tiles cost.  Every warp sums up the lengths by itself (its CTA
 // does, before the first load) and finds its range there.  A unit that lies in one warp's range is written at once; a unit
 // cut by ranges leaves (o, m, l, sum of gates) of every part in a workspace, which a second kernel joins.
 //
@@ -40,7 +41,8 @@ __host__ __device__ constexpr int pag_warps(int64_t D) { return D == 128 ? 8 : 1
 __host__ __device__ constexpr int pag_ranges(int64_t D) { return kPagGrid * pag_warps(D); }
 constexpr int kPagTile = 16;
 constexpr int kPagRows = 8;          // query heads of a unit
-constexpr int kPagLeastTiles = 2;    // of a range
+constexpr int kPagStart = 2;         // what the start of a unit costs, in tiles
+constexpr int kPagLeast = 4;         // of a range, starts counted
 constexpr int kPagSite = 95;           // of a wait that ran out
 constexpr float kPagLog2e = 1.4426950408889634f, kPagLn2 = 0.6931471805599453f;
 
@@ -67,8 +69,10 @@ __device__ __forceinline__ int pag_length(const PagedParams& p, int r) {
 template <int D>
 __device__ __forceinline__ int64_t pag_per_range(int64_t tiles) {
   const int64_t per = (tiles + pag_ranges(D) - 1) / pag_ranges(D);
-  return per < kPagLeastTiles ? kPagLeastTiles : per;
+  return per < kPagLeast ? kPagLeast : per;
 }
+// a request's length in the row of tiles, for one unit
+__device__ __forceinline__ int pag_places(int length) { return length ? (length + kPagTile - 1) / kPagTile + kPagStart : 0; }
 
 template <bool kBf16>
 __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -89,6 +93,12 @@ __device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
+}
+
+// Asks L1 for what will be loaded from here in a while.
+__device__ __forceinline__ void touch(const void* p) {
+  uint16_t unused;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(p) : "memory");
 }
 
 template <int D>
@@ -137,7 +147,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   const int share = (p.R + kThreads - 1) / kThreads;
   const int r_first = min(tid * share, p.R), r_end = min(r_first + share, p.R);
   int64_t mine = 0;
-  for (int r = r_first; r < r_end; ++r) mine += (pag_length(p, r) + kPagTile - 1) / kPagTile;
+  for (int r = r_first; r < r_end; ++r) mine += pag_places(pag_length(p, r));
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -155,7 +165,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     int64_t at = incl - mine;
     for (int r = r_first; r < r_end; ++r) {
       p.tiles_before[r] = at;
-      at += (pag_length(p, r) + kPagTile - 1) / kPagTile;
+      at += pag_places(pag_length(p, r));
     }
     if (tid == 0) p.tiles_before[p.R] = s_before[kThreads];
   }
@@ -171,10 +181,9 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   const int range = warp * gridDim.x + blockIdx.x;
   const int64_t t_begin = range * per, t_end = min(t_begin + per, total);
   if (t_begin >= t_end) return;
-  // (a range is far below 2^31 tiles: 2^31 keys of 65535 requests' heads, cut by more than a thousand)
-  int left = static_cast<int>(min(t_end - t_begin, static_cast<int64_t>(2147483647)));   // tiles to ask for
-  int n_left = left;                                                                     // tiles to use
-  int r, unit, n_tiles, part_lo, at, length, flags, kh, h0, heads;   // the part being asked for: tiles part_lo .. of a unit, next `at`
+  // (a range is far below 2^31 places: 2^31 keys of 65535 requests' heads, cut by more than a thousand)
+  int left = static_cast<int>(min(t_end - t_begin, static_cast<int64_t>(2147483647)));   // places not yet gone through
+  int r, unit, n_tiles, place, at, part_lo = 0, length, flags = 0, kh, h0, heads;        // the part asked for: tiles part_lo .. at
   {
     int lo = 0, hi = kThreads;      // the last share that begins at or before the range
     while (hi - lo > 1) {
@@ -183,25 +192,30 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
       else hi = mid;
     }
     int64_t before = s_before[lo];
+    int places;
     r = lo * share;
     for (;; ++r) {
       length = pag_length(p, r);
-      n_tiles = (length + kPagTile - 1) / kPagTile;
-      if ((before + n_tiles) * p.units > t_begin) break;
-      before += n_tiles;
+      places = pag_places(length);
+      if ((before + places) * p.units > t_begin) break;
+      before += places;
     }
+    n_tiles = places - kPagStart;
     const int64_t off = t_begin - before * p.units;
-    unit = static_cast<int>(off / n_tiles);
-    part_lo = static_cast<int>(off - static_cast<int64_t>(unit) * n_tiles);
+    unit = static_cast<int>(off / places);
+    place = static_cast<int>(off - static_cast<int64_t>(unit) * places);
   }
-  auto begin_part = [&](int second) {   // from part_lo on, as far as the range goes
-    const int hi = n_tiles - part_lo < left ? n_tiles : part_lo + left;
+  // the unit's part from `place` on, as far as the range goes; none (at < part_lo) where it ends inside the unit's start
+  auto begin_part = [&](int second) {
+    const int take = min(n_tiles + kPagStart - place, left);
     kh = unit / p.tiles_of_group;
     const int in_group = (unit - kh * p.tiles_of_group) * kPagRows;
     h0 = kh * p.group + in_group;
     heads = min(p.group - in_group, kPagRows);
-    flags = kItemFirst | second | (part_lo == 0 && hi == n_tiles ? kItemWhole : 0) | heads << 8;
-    at = hi - 1;
+    part_lo = max(place - kPagStart, 0);
+    at = max(place + take - kPagStart, 0) - 1;
+    left -= take;
+    flags = kItemFirst | second | (part_lo == 0 && at == n_tiles - 1 ? kItemWhole : 0) | heads << 8;
   };
   begin_part(0);
 
@@ -218,8 +232,9 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   int page_r = -1, page_base = 0, page_ids = -1;   // 32 entries of a request's table row, one to a lane
 
   int ask_stage = 0;
+  int pending = 0;   // tiles asked for and not yet used
   auto ask = [&]() {   // the next tile
-    if (left <= 0) return;
+    if (at < part_lo) return;
     const int key0 = at * kPagTile, j = key0 >> p.page_log2, row0 = key0 & ((1 << p.page_log2) - 1);
     if (r != page_r || j < page_base || j >= page_base + 32) {
       page_r = r;
@@ -248,16 +263,17 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     if (there && lane < heads)
       bulk_load(ring_g + ask_stage * (Tile::kGates / 4) + lane * kPagTile, p.gates + id * p.g_sp + (h0 + lane) * p.g_sh + row0,
                 kPagTile * 4, bar);
+    if ((flags & kItemFirst) && x < heads) touch(p.q + r * p.q_sr + (h0 + x) * p.q_sh + (D == 16 ? c * 4 : D == 32 ? c * 8 : c * 16));
     flags &= ~kItemFirst;
+    ++pending;
     --at;
-    --left;
     if (last && left > 0) {   // the next unit
-      part_lo = 0;
+      place = 0;
       if (++unit == p.units) {
         unit = 0;
         do {
           length = pag_length(p, ++r);
-        } while (length == 0);   // (tiles are left, so there is a request with keys)
+        } while (length == 0);   // (places are left, so there is a request with keys)
         n_tiles = (length + kPagTile - 1) / kPagTile;
       }
       begin_part(kItemSecond);
@@ -279,9 +295,11 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   float o[Tile::kCols][4], m = -INFINITY, l = 0.f, carry = 0.f;
   int stage = 0;
   uint32_t parity = 0;
-  for (; n_left > 0; --n_left) {
+  for (;;) {
     ask();
-    if (!mbar_wait_warp(&s_full[warp][stage], parity, &s_abort, p.status, kPagSite, n_left)) break;
+    if (pending == 0) break;
+    if (!mbar_wait_warp(&s_full[warp][stage], parity, &s_abort, p.status, kPagSite, pending)) break;
+    --pending;
     __syncwarp();
     const PagedItem item = s_item[warp][stage];
     const uint32_t tile = ring_u32 + stage * Tile::kStage;
@@ -415,10 +433,9 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
       parity ^= 1;
     }
   }
-  if (n_left > 0) {   // gave up: the copies that are still in flight end before their memory does
+  if (pending > 0) {   // gave up: the copies that are still in flight end before their memory does
     volatile int none = 0;
-    const int asked = n_left - left;
-    for (int i = 0; i < asked; ++i) {
+    for (; pending > 0; --pending) {
       mbar_wait_warp(&s_full[warp][stage], parity, &none, p.status, kPagSite, -1);
       none = 0;
       if (++stage == kStages) {
@@ -429,75 +446,101 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   }
 }
 
-// Joins the parts of units that were cut.  A CTA takes (request, query head) pairs; a unit's parts stand from the left, so
-// their gate sums are added from the right, 32 parts at a time by one warp; then 256 / D groups of threads each sum every
-// (256 / D)-th part.
+// Joins the parts of units that were cut.  A CTA takes (request, query head) pairs.  A unit's parts stand from the left: their
+// gate sums are added from the right by one warp, 32 parts at a time.  kLanes lanes share a part's channels, the kGroups groups of
+// threads each take every kGroups-th part; the first kAhead of these are asked for before the weights are known.
 template <bool kBf16, int D>
 __global__ void __launch_bounds__(256) fox_paged_join_kernel(const PagedParams p) {
-  __shared__ float s_w[pag_ranges(D)], s_o[256], s_top, s_sum;
-  constexpr int kGroups = 256 / D;
-  const int tid = threadIdx.x;
+  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kAhead = 6;
+  __shared__ float s_w[pag_ranges(D)], s_l[pag_ranges(D)], s_g[pag_ranges(D)], s_sum, s_top;
+  __shared__ float4 s_o[256];
+  const int tid = threadIdx.x, sub = tid % kLanes, g0 = tid / kLanes;
   wait_for_kernel_in_front();
   const int64_t per = pag_per_range<D>(p.tiles_before[p.R] * p.units);
   for (int64_t item = blockIdx.x; item < static_cast<int64_t>(p.R) * p.H; item += gridDim.x) {
     const int r = static_cast<int>(item / p.H), h = static_cast<int>(item - static_cast<int64_t>(r) * p.H);
     const int kh = h / p.group, row = h - kh * p.group, unit = kh * p.tiles_of_group + row / kPagRows;
-    const int64_t before = p.tiles_before[r], n_tiles = p.tiles_before[r + 1] - before;
-    const int64_t u0 = before * p.units + unit * n_tiles, u1 = u0 + n_tiles;
-    if (n_tiles == 0) continue;
-    const int w0 = static_cast<int>(u0 / per), n = static_cast<int>((u1 - 1) / per) - w0 + 1;   // (at most all ranges)
+    const int64_t before = p.tiles_before[r], places = p.tiles_before[r + 1] - before;
+    if (places == 0) continue;
+    const int64_t u0 = before * p.units + unit * places;
+    const int w0 = static_cast<int>((u0 + kPagStart) / per), n = static_cast<int>((u0 + places - 1) / per) - w0 + 1;   // (at most all ranges)
     if (n == 1) continue;
     const int64_t ld = static_cast<int64_t>(p.rows) * (D + 4);
     const float* base = p.part + (static_cast<int64_t>(w0) * 2 * p.rows + row % kPagRows) * (D + 4);
-    const int second = u0 != w0 * per;   // the first part's place
+    const int second = w0 * per < u0;   // the first part's place: its range has begun in another unit
     auto at = [&](int s) { return base + (2 * s + (s == 0 ? second : 0)) * ld; };
+    float4 ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = g0 + i * kGroups;
+      ahead[i] = s < n ? *reinterpret_cast<const float4*>(at(s) + sub * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int s = tid; s < n; s += 256) {
+      const float4 v = *reinterpret_cast<const float4*>(at(s) + D);
+      s_w[s] = v.x;
+      s_l[s] = v.y;
+      s_g[s] = v.z;
+    }
+    __syncthreads();
     if (tid < 32) {
       float after = 0.f, top = -INFINITY;
       for (int e = n; e > 0; e -= 32) {   // parts e - 1 - lane
         const int s = e - 1 - tid;
-        const float g = s >= 0 ? at(s)[D + 2] : 0.f;
-        float incl = g;
+        float incl = s >= 0 ? s_g[s] : 0.f;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const float y = __shfl_up_sync(0xffffffffu, incl, o);
           if (tid >= o) incl += y;
         }
-        const float right = __shfl_up_sync(0xffffffffu, incl, 1);
+        const float right = __shfl_up_sync(0xffffffffu, incl, 1);   // (not incl less its own: that may be minus infinity)
         if (s >= 0) {
-          const float mm = at(s)[D] + after + (tid ? right : 0.f);
+          const float mm = s_w[s] + (tid ? after + right : after);
           s_w[s] = mm;
           top = fmaxf(top, mm);
         }
         after += __shfl_sync(0xffffffffu, incl, 31);
       }
+#pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       float sum = 0.f;
       for (int s = n - 1 - tid; s >= 0; s -= 32) {   // (each lane those that it wrote)
-        const float mm = s_w[s], w = mm == -INFINITY ? 0.f : fast_exp2(mm - top), ls = at(s)[D + 1];
+        const float mm = s_w[s], w = mm == -INFINITY ? 0.f : fast_exp2(mm - top);
         s_w[s] = w;
-        sum = fmaf(ls, w, sum);
+        sum = fmaf(s_l[s], w, sum);
       }
+#pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (tid == 0) {
-        s_top = top;
         s_sum = sum;
+        s_top = top;
       }
     }
     __syncthreads();
-    const int d = tid % D, g0 = tid / D;
-    float a = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](const float4& v, float w) {   // (a weight of zero too: a NaN value counts)
+      a.x = fmaf(v.x, w, a.x);
+      a.y = fmaf(v.y, w, a.y);
+      a.z = fmaf(v.z, w, a.z);
+      a.w = fmaf(v.w, w, a.w);
+    };
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int s = g0 + i * kGroups;
+      if (s < n) add(ahead[i], s_w[s]);
+    }
 #pragma unroll 4
-    for (int s = g0; s < n; s += kGroups) a = fmaf(at(s)[d], s_w[s], a);   // (a weight of zero too: a NaN value counts)
+    for (int s = g0 + kAhead * kGroups; s < n; s += kGroups) add(*reinterpret_cast<const float4*>(at(s) + sub * 4), s_w[s]);
     s_o[tid] = a;
     __syncthreads();
-    if (tid < D) {
+    if (tid < kLanes) {
 #pragma unroll
-      for (int g = 1; g < kGroups; ++g) a += s_o[g * D + tid];
-      const uint32_t pk = pack2<kBf16>(s_sum != 0.f ? a / s_sum : 0.f, 0.f);
-      p.o[r * p.o_sr + h * p.o_sh + tid] = static_cast<uint16_t>(pk & 0xffffu);
+      for (int g = 1; g < kGroups; ++g) add(s_o[g * kLanes + tid], 1.f);
+      const float inv = s_sum != 0.f ? 1.f / s_sum : 0.f;
+      *reinterpret_cast<uint2*>(p.o + r * p.o_sr + h * p.o_sh + tid * 4) =
+          make_uint2(pack2<kBf16>(a.x * inv, a.y * inv), pack2<kBf16>(a.z * inv, a.w * inv));
     }
     if (tid == 0 && p.L) p.L[item] = s_sum != 0.f ? s_top * kPagLn2 + __logf(s_sum) : -INFINITY;
-    __syncthreads();   // (s_w, s_o: the next pair's)
+    __syncthreads();   // (what is shared: the next pair's)
   }
 }
 
