@@ -7,10 +7,11 @@
 //
 // Work is counted in tiles of 16 keys of one unit (a request and a key head, with up to 8 of the query heads that share it).
 // All tiles of all units stand in one row, with kPagStart places more in front of each unit for what its start costs; the row is
-// cut into equal ranges, one for each warp of a grid that fills the GPU once: the longest request and the shortest cost what
-// their tiles cost.  Every warp sums up the lengths by itself (its CTA
-// does, before the first load) and finds its range there.  A unit that lies in one warp's range is written at once; a unit
-// cut by ranges leaves (o, m, l, sum of gates) of every part in a workspace, which a second kernel joins.
+// cut into equal ranges for the CTAs of a grid that fills the GPU once, and each of these into equal ranges for its warps: the
+// longest request and the shortest cost what their tiles cost.  Every CTA sums up the lengths by itself before its first load and
+// finds its range there.  A unit of a few hundred keys is not cut between CTAs (its range is moved to the unit's end).  A unit
+// that lies in one warp's range is written at once; of one that is cut, each part's (o, m, l, sum of gates) goes to a workspace.
+// The CTA joins its warps' parts at its end, a second kernel the CTAs' parts.
 //
 // The bias of a key is the sum of the gates behind it.  A warp goes through its part of a unit from the right, so that this
 // is a running sum (exact where the bias is small, which is where it matters; a prefix sum over the whole request would lose
@@ -38,11 +39,13 @@ namespace fox {
 
 constexpr int kPagGrid = kSms;
 __host__ __device__ constexpr int pag_warps(int64_t D) { return D == 128 ? 8 : 16; }
-__host__ __device__ constexpr int pag_ranges(int64_t D) { return kPagGrid * pag_warps(D); }
 constexpr int kPagTile = 16;
 constexpr int kPagRows = 8;          // query heads of a unit
 constexpr int kPagStart = 2;         // what the start of a unit costs, in tiles
-constexpr int kPagLeast = 4;         // of a range, starts counted
+constexpr int kPagLeast = 3;         // places of a warp
+// Units of up to so many places are one CTA's: some 280 KB of keys and values, which one SM reads in the time that parts of several
+// CTAs take to be joined.
+__host__ __device__ constexpr int pag_whole(int64_t D) { return (D == 128 ? 32 : 64) + kPagStart; }
 constexpr int kPagSite = 95;           // of a wait that ran out
 constexpr float kPagLog2e = 1.4426950408889634f, kPagLn2 = 0.6931471805599453f;
 
@@ -54,10 +57,11 @@ struct PagedParams {
   int64_t table_ld;
   uint16_t* o;
   float* L;                            // (R, H) or nullptr
-  float* part;                         // (ranges, 2, rows, D + 4)
-  int64_t* tiles_before;               // (R + 1)
+  float* part;                         // (CTAs, 2, rows, D + 4), then (CTAs, warps, 2, rows, D + 4)
+  int* before;                         // (R + 1): places of a unit in front of every request
   int R, H, group, rows, tiles_of_group, units, n_pages, page_log2;   // rows: of a unit; units: of a request
   int32_t* status;
+  Divisor by_units, by_tiles_of_group;
   int64_t most;                        // keys that a table row has entries for
   float qk_scale;                      // sm_scale * log2(e)
 };
@@ -66,13 +70,29 @@ __device__ __forceinline__ int pag_length(const PagedParams& p, int r) {
   const int64_t n = p.lengths[r];
   return static_cast<int>(n < 0 ? 0 : n < p.most ? n : p.most);
 }
-template <int D>
-__device__ __forceinline__ int64_t pag_per_range(int64_t tiles) {
-  const int64_t per = (tiles + pag_ranges(D) - 1) / pag_ranges(D);
-  return per < kPagLeast ? kPagLeast : per;
+__device__ __forceinline__ int pag_per_cta(int places) { return (places + kPagGrid - 1) / kPagGrid; }
+// t / d (an integer division is forty instructions): the product is off by less than 2 for quotients below 2^22
+__device__ __forceinline__ int pag_div(int t, int d) {
+  int q = static_cast<int>(static_cast<float>(t) * __frcp_rn(static_cast<float>(d)));
+  int left = static_cast<int>(static_cast<uint32_t>(t) - static_cast<uint32_t>(q) * static_cast<uint32_t>(d));
+  while (left < 0) {
+    left += d;
+    --q;
+  }
+  while (left >= d) {
+    left -= d;
+    ++q;
+  }
+  return q;
 }
 // a request's length in the row of tiles, for one unit
 __device__ __forceinline__ int pag_places(int length) { return length ? (length + kPagTile - 1) / kPagTile + kPagStart : 0; }
+
+// Asks L1 for what will be loaded from here in a while.
+__device__ __forceinline__ void touch(const void* p) {
+  uint16_t unused;
+  asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(p) : "memory");
+}
 
 template <bool kBf16>
 __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -95,12 +115,6 @@ __device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
   return v;
 }
 
-// Asks L1 for what will be loaded from here in a while.
-__device__ __forceinline__ void touch(const void* p) {
-  uint16_t unused;
-  asm volatile("ld.global.u16 %0, [%1];" : "=h"(unused) : "l"(p) : "memory");
-}
-
 template <int D>
 struct PagedTile {
   static constexpr int kHalves = D == 128 ? 2 : 1;            // boxes of 16 keys x 64 columns
@@ -119,6 +133,10 @@ struct PagedItem {
 };
 enum { kItemFirst = 1, kItemLast = 2, kItemWhole = 4, kItemSecond = 8 };   // of its part; a unit's only part; workspace place 1
 
+struct PagedUnit {
+  int r, unit, at, places, length;   // at: its first place in the row
+};
+
 template <bool kBf16, int D>
 __global__ void __launch_bounds__(PagedTile<D>::kThreads, 1)
 fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
@@ -127,8 +145,11 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   extern __shared__ __align__(1024) char pag_smem[];
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ int s_abort;
-  __shared__ int64_t s_before[kThreads + 1];
-  __shared__ int64_t s_warp[kWarps];
+  __shared__ int s_before[kThreads + 1];
+  __shared__ int s_length[kThreads];
+  __shared__ PagedUnit s_unit[kWarps + 1];   // that the warps' ranges begin in; that the CTA's ends in
+  __shared__ int s_range[3];
+  __shared__ int s_warp[kWarps];
   __shared__ PagedItem s_item[kWarps][kStages];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (lane == 0) {
@@ -143,72 +164,103 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   wait_for_kernel_in_front();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the joining kernel, which waits for this one's end)
 
-  // ---- where every thread's share of the requests begins in the row of tiles
+  // ---- where every thread's share of the requests begins in the row of places
   const int share = (p.R + kThreads - 1) / kThreads;
   const int r_first = min(tid * share, p.R), r_end = min(r_first + share, p.R);
-  int64_t mine = 0;
-  for (int r = r_first; r < r_end; ++r) mine += pag_places(pag_length(p, r));
-  int64_t incl = mine;
+  int mine = 0;
+  for (int r = r_first; r < r_end; ++r) {
+    const int n = pag_length(p, r);
+    s_length[tid] = n;   // (used where a share is one request)
+    if (share == 1 && n) touch(p.table + r * p.table_ld + ((n - 1) >> p.page_log2));   // (where its pages will be looked up first)
+    mine += pag_places(n);
+  }
+  int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
     if (lane >= o) incl += y;
   }
   if (lane == 31) s_warp[warp] = incl;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) incl += s_warp[w];
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w)
+    if (w < warp) incl += s_warp[w];
   s_before[tid + 1] = incl;
   if (tid == 0) s_before[0] = 0;
   __syncthreads();
-  const int64_t total = s_before[kThreads] * p.units, per = pag_per_range<D>(total);
   if (blockIdx.x == 0) {
-    int64_t at = incl - mine;
+    int at = incl - mine;
     for (int r = r_first; r < r_end; ++r) {
-      p.tiles_before[r] = at;
+      p.before[r] = at;
       at += pag_places(pag_length(p, r));
     }
-    if (tid == 0) p.tiles_before[p.R] = s_before[kThreads];
+    if (tid == 0) p.before[p.R] = s_before[kThreads];
   }
   // ---- requests without a key
   for (int r = blockIdx.x; r < p.R; r += gridDim.x) {
-    if (pag_length(p, r)) continue;
+    if (share == 1 ? s_length[r] : pag_length(p, r)) continue;
     for (int i = tid; i < p.H * D; i += kThreads) p.o[r * p.o_sr + (i / D) * p.o_sh + i % D] = 0;
     if (p.L)
       for (int h = tid; h < p.H; h += kThreads) p.L[static_cast<int64_t>(r) * p.H + h] = -INFINITY;
   }
+  const int total = s_before[kThreads] * p.units, per_cta = pag_per_cta(total), raw = min(static_cast<int>(blockIdx.x) * per_cta, total);   // (148 * per_cta is below 2^30 + 148)
 
-  // ---- this warp's range (neighbours in the row on different SMs, so that little work is on many)
-  const int range = warp * gridDim.x + blockIdx.x;
-  const int64_t t_begin = range * per, t_end = min(t_begin + per, total);
-  if (t_begin >= t_end) return;
-  // (a range is far below 2^31 places: 2^31 keys of 65535 requests' heads, cut by more than a thousand)
-  int left = static_cast<int>(min(t_end - t_begin, static_cast<int64_t>(2147483647)));   // places not yet gone through
-  int r, unit, n_tiles, place, at, part_lo = 0, length, flags = 0, kh, h0, heads;        // the part asked for: tiles part_lo .. at
-  {
-    int lo = 0, hi = kThreads;      // the last share that begins at or before the range
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_before[mid] * p.units <= t_begin) lo = mid;
-      else hi = mid;
+  // ---- this CTA's range, moved to the ends of units that are not cut, and in it those of its warps: by one warp, a place to a lane
+  if (warp == 0) {
+    auto find = [&](int t) {   // the unit that place t (< total) of the row belongs to
+      const int q = div_by(p.by_units, t);
+      int lo = 0;   // the last share that begins at or before q
+#pragma unroll
+      for (int s = kThreads / 2; s > 0; s >>= 1)
+        if (s_before[lo + s] <= q) lo += s;
+      int before = s_before[lo];
+      PagedUnit f;
+      f.r = lo * share;
+      f.length = share == 1 ? s_length[lo] : pag_length(p, f.r);
+      f.places = pag_places(f.length);
+      while (before + f.places <= q) {
+        before += f.places;
+        f.length = pag_length(p, ++f.r);
+        f.places = pag_places(f.length);
+      }
+      const int off = t - before * p.units;
+      f.unit = pag_div(off, f.places);
+      f.at = before * p.units + f.unit * f.places;
+      return f;
+    };
+    int edge = lane ? min(raw + per_cta, total) : raw;   // lane 0: where the range begins; the others: where it ends
+    if (edge < total) {
+      const PagedUnit f = find(edge);
+      if (f.at < edge && f.places <= pag_whole(D)) edge = f.at + f.places;
     }
-    int64_t before = s_before[lo];
-    int places;
-    r = lo * share;
-    for (;; ++r) {
-      length = pag_length(p, r);
-      places = pag_places(length);
-      if ((before + places) * p.units > t_begin) break;
-      before += places;
+    const int c_begin = __shfl_sync(0xffffffffu, edge, 0), c_end = __shfl_sync(0xffffffffu, edge, 1);
+    const int per = max((c_end - c_begin + kWarps - 1) / kWarps, kPagLeast);
+    const int t = lane < kWarps ? c_begin + lane * per : c_end - 1;   // (the last: the unit that the range ends in)
+    if (lane <= kWarps && t < c_end && c_begin < c_end) s_unit[lane] = find(t);
+    if (lane == 0) {
+      s_range[0] = c_begin;
+      s_range[1] = c_end;
+      s_range[2] = per;
     }
-    n_tiles = places - kPagStart;
-    const int64_t off = t_begin - before * p.units;
-    unit = static_cast<int>(off / places);
-    place = static_cast<int>(off - static_cast<int64_t>(unit) * places);
+  }
+  __syncthreads();
+  const int c_begin = s_range[0], c_end = s_range[1], per = s_range[2];
+  if (c_begin >= c_end) return;
+  const int t_begin = min(c_begin + warp * per, c_end);
+  int r = 0, unit = 0, n_tiles = 0, place = 0, at = -1, part_lo = 0, length = 0, flags = 0, kh = 0, h0 = 0, heads = 0;   // the part asked for: tiles part_lo .. at
+  int left = min(per, c_end - t_begin);   // places not yet gone through
+  if (left > 0) {
+    const PagedUnit f = s_unit[warp];
+    r = f.r;
+    unit = f.unit;
+    place = t_begin - f.at;
+    length = f.length;
+    n_tiles = f.places - kPagStart;
   }
   // the unit's part from `place` on, as far as the range goes; none (at < part_lo) where it ends inside the unit's start
   auto begin_part = [&](int second) {
     const int take = min(n_tiles + kPagStart - place, left);
-    kh = unit / p.tiles_of_group;
+    kh = div_by(p.by_tiles_of_group, unit);
     const int in_group = (unit - kh * p.tiles_of_group) * kPagRows;
     h0 = kh * p.group + in_group;
     heads = min(p.group - in_group, kPagRows);
@@ -217,7 +269,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     left -= take;
     flags = kItemFirst | second | (part_lo == 0 && at == n_tiles - 1 ? kItemWhole : 0) | heads << 8;
   };
-  begin_part(0);
+  if (left > 0) begin_part(0);
 
   const uint32_t smem0 = (smem_u32(pag_smem) + 1023) & ~1023u;
   char* const base = pag_smem + (smem0 - smem_u32(pag_smem));
@@ -415,7 +467,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
             *reinterpret_cast<uint32_t*>(to + j * 8 + 2 * c) = pack2<kBf16>((o[j][0] + o[j][2]) * inv, (o[j][1] + o[j][3]) * inv);
           if (p.L && c == 0) p.L[static_cast<int64_t>(item.r) * p.H + h] = ls != 0.f ? m_ref * kPagLn2 + __logf(ls) : -INFINITY;
         } else {
-          float* to = p.part + ((static_cast<int64_t>(range) * 2 + (item.flags & kItemSecond ? 1 : 0)) * p.rows + x) * (D + 4);
+          float* to = p.part + ((static_cast<int64_t>(2 * kPagGrid) + (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * 2 + (item.flags & kItemSecond ? 1 : 0)) * p.rows + x) * (D + 4);
 #pragma unroll
           for (int j = 0; j < Tile::kCols; ++j)
             *reinterpret_cast<float2*>(to + j * 8 + 2 * c) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
@@ -444,30 +496,124 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
       }
     }
   }
+  // ---- the parts of this CTA's warps joined: those of the unit that a warp's range begins in, where it ends in that range or the
+  // CTA's range ends there, and those of the unit that the CTA's range ends in.  A unit that other CTAs have a part of becomes one
+  // part of this CTA's.  The query heads of these units go around the warps.
+  __syncthreads();
+  for (int i = warp; i < (kWarps + 1) * p.rows; i += kWarps) {
+    const int row_j = i / (kWarps + 1), of = i - row_j * (kWarps + 1);
+    const int b = of < kWarps ? c_begin + of * per : c_end - 1, e = min(b + per, c_end);
+    if (b >= c_end) continue;
+    const PagedUnit f = s_unit[of];
+    if (of < kWarps ? f.at + f.places > e && e != c_end : f.at <= c_begin + pag_div(c_end - 1 - c_begin, per) * per) continue;   // (the first unit of
+                                                                                                       // the last range has its turn as that)
+    const int first = max(f.at + kPagStart, c_begin), last = min(f.at + f.places, c_end) - 1;   // of its places with tiles here
+    if (first > last) continue;
+    const int wa = pag_div(first - c_begin, per), n = pag_div(last - c_begin, per) - wa + 1;
+    const bool here = f.at + kPagStart >= c_begin && f.at + f.places <= c_end;   // all of its tiles
+    if (here && n == 1) continue;   // (written where it was computed)
+    const int kh_j = div_by(p.by_tiles_of_group, f.unit), in_group = (f.unit - kh_j * p.tiles_of_group) * kPagRows;
+    const int h_j = kh_j * p.group + in_group + row_j;
+    if (row_j >= p.group - in_group) continue;
+    const int64_t rows_ld = static_cast<int64_t>(p.rows) * (D + 4);
+    const float* from = p.part + (2 * kPagGrid + (static_cast<int64_t>(blockIdx.x) * kWarps + wa) * 2) * rows_ld + row_j * (D + 4);
+    const bool second = c_begin + wa * per < f.at;   // the first part's place: its warp has begun in another unit
+    auto part = [&](int s) { return from + 2 * s * rows_ld + (s == 0 && second ? rows_ld : 0); };
+    // lane s: part s
+    float4 st = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    if (lane < n) st = *reinterpret_cast<const float4*>(part(lane) + D);
+    constexpr int kPer = D / 32 > 0 ? D / 32 : 1;   // channels of a lane
+    float v[kWarps][kPer];
+#pragma unroll
+    for (int s = 0; s < kWarps; ++s) {
+      const float* at_v = part(s) + lane * kPer;
+      const bool in = s < n && lane * kPer < D;
+      if constexpr (kPer == 4) {
+        const float4 x4 = in ? *reinterpret_cast<const float4*>(at_v) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[s][0] = x4.x; v[s][1] = x4.y; v[s][2] = x4.z; v[s][3] = x4.w;
+      } else if constexpr (kPer == 2) {
+        const float2 x2 = in ? *reinterpret_cast<const float2*>(at_v) : make_float2(0.f, 0.f);
+        v[s][0] = x2.x; v[s][1] = x2.y;
+      } else {
+        v[s][0] = in ? *at_v : 0.f;
+      }
+    }
+    float behind = st.z, y;   // gates of the parts from this one on
+#pragma unroll
+    for (int o = 1; o < kWarps; o <<= 1) {
+      y = __shfl_down_sync(0xffffffffu, behind, o);
+      if (lane + o < kWarps) behind += y;
+    }
+    const float all = __shfl_sync(0xffffffffu, behind, 0);
+    y = __shfl_down_sync(0xffffffffu, behind, 1);
+    const float mm = lane < n ? st.x + (lane + 1 < kWarps ? y : 0.f) : -INFINITY;
+    float top = mm;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float w = mm == -INFINITY ? 0.f : fast_exp2(mm - top);   // (NaN stays)
+    float sum = st.y * w;
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    float acc[kPer];
+#pragma unroll
+    for (int c_i = 0; c_i < kPer; ++c_i) acc[c_i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < kWarps; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+#pragma unroll
+      for (int c_i = 0; c_i < kPer; ++c_i)
+        if (s < n) acc[c_i] = fmaf(v[s][c_i], ws, acc[c_i]);   // (a weight of zero too: a NaN value counts)
+    }
+    sum = __shfl_sync(0xffffffffu, sum, 0);
+    top = __shfl_sync(0xffffffffu, top, 0);
+    if (here) {
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      uint16_t* to = p.o + f.r * p.o_sr + h_j * p.o_sh + lane * kPer;
+      if (lane * kPer < D) {
+        if constexpr (kPer == 1) {
+          *to = static_cast<uint16_t>(pack2<kBf16>(acc[0] * inv, 0.f) & 0xffffu);
+        } else {
+#pragma unroll
+          for (int c_i = 0; c_i < kPer; c_i += 2) *reinterpret_cast<uint32_t*>(to + c_i) = pack2<kBf16>(acc[c_i] * inv, acc[c_i + 1] * inv);
+        }
+      }
+      if (p.L && lane == 0) p.L[static_cast<int64_t>(f.r) * p.H + h_j] = sum != 0.f ? top * kPagLn2 + __logf(sum) : -INFINITY;
+    } else {
+      float* to = p.part + (static_cast<int64_t>(blockIdx.x) * 2 + (raw < f.at ? 1 : 0)) * rows_ld + row_j * (D + 4);
+      if (lane * kPer < D)
+#pragma unroll
+        for (int c_i = 0; c_i < kPer; ++c_i) to[lane * kPer + c_i] = acc[c_i];
+      if (lane == 0) *reinterpret_cast<float4*>(to + D) = make_float4(sum != sum ? sum : top, sum, all, 0.f);
+    }
+  }
 }
 
-// Joins the parts of units that were cut.  A CTA takes (request, query head) pairs.  A unit's parts stand from the left: their
-// gate sums are added from the right by one warp, 32 parts at a time.  kLanes lanes share a part's channels, the kGroups groups of
-// threads each take every kGroups-th part; the first kAhead of these are asked for before the weights are known.
+// Joins the CTAs' parts of units that several CTAs have a part of.  A CTA here takes (request, query head) pairs.  A unit's parts
+// stand from the left: their gate sums are added from the right by one warp, 32 parts at a time.  kLanes lanes share a part's
+// channels, the kGroups groups of threads each take every kGroups-th part; the first kAhead of these are asked for before the weights
+// are known.
+constexpr int kJoinThreads = 128;
 template <bool kBf16, int D>
-__global__ void __launch_bounds__(256) fox_paged_join_kernel(const PagedParams p) {
-  constexpr int kLanes = D / 4, kGroups = 256 / kLanes, kAhead = 6;
-  __shared__ float s_w[pag_ranges(D)], s_l[pag_ranges(D)], s_g[pag_ranges(D)], s_sum, s_top;
-  __shared__ float4 s_o[256];
+__global__ void __launch_bounds__(kJoinThreads) fox_paged_join_kernel(const PagedParams p) {
+  constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAhead = 8;
+  __shared__ float s_w[kPagGrid], s_l[kPagGrid], s_g[kPagGrid], s_sum, s_top;
+  __shared__ float4 s_o[kJoinThreads];
   const int tid = threadIdx.x, sub = tid % kLanes, g0 = tid / kLanes;
   wait_for_kernel_in_front();
-  const int64_t per = pag_per_range<D>(p.tiles_before[p.R] * p.units);
+  const int per = pag_per_cta(p.before[p.R] * p.units);
   for (int64_t item = blockIdx.x; item < static_cast<int64_t>(p.R) * p.H; item += gridDim.x) {
-    const int r = static_cast<int>(item / p.H), h = static_cast<int>(item - static_cast<int64_t>(r) * p.H);
+    const int r = static_cast<int>(item < (int64_t{1} << 31) ? static_cast<uint32_t>(item) / static_cast<uint32_t>(p.H) : item / p.H);
+    const int h = static_cast<int>(item - static_cast<int64_t>(r) * p.H);
+    const int before = p.before[r];
+    const int places = pag_places(pag_length(p, r));
+    if (places <= pag_whole(D)) continue;
     const int kh = h / p.group, row = h - kh * p.group, unit = kh * p.tiles_of_group + row / kPagRows;
-    const int64_t before = p.tiles_before[r], places = p.tiles_before[r + 1] - before;
-    if (places == 0) continue;
-    const int64_t u0 = before * p.units + unit * places;
-    const int w0 = static_cast<int>((u0 + kPagStart) / per), n = static_cast<int>((u0 + places - 1) / per) - w0 + 1;   // (at most all ranges)
+    const int u0 = before * p.units + unit * places;
+    const int w0 = pag_div(u0 + kPagStart, per), n = pag_div(u0 + places - 1, per) - w0 + 1;
     if (n == 1) continue;
     const int64_t ld = static_cast<int64_t>(p.rows) * (D + 4);
     const float* base = p.part + (static_cast<int64_t>(w0) * 2 * p.rows + row % kPagRows) * (D + 4);
-    const int second = w0 * per < u0;   // the first part's place: its range has begun in another unit
+    const int second = w0 * per < u0;   // the first part's place: its CTA's range has begun in another unit
     auto at = [&](int s) { return base + (2 * s + (s == 0 ? second : 0)) * ld; };
     float4 ahead[kAhead];
 #pragma unroll
@@ -475,7 +621,7 @@ __global__ void __launch_bounds__(256) fox_paged_join_kernel(const PagedParams p
       const int s = g0 + i * kGroups;
       ahead[i] = s < n ? *reinterpret_cast<const float4*>(at(s) + sub * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    for (int s = tid; s < n; s += 256) {
+    for (int s = tid; s < n; s += kJoinThreads) {
       const float4 v = *reinterpret_cast<const float4*>(at(s) + D);
       s_w[s] = v.x;
       s_l[s] = v.y;
@@ -554,13 +700,17 @@ static int launch_paged(const PagedParams& p, const CUtensorMap& map_k, const CU
     if (cudaFuncSetAttribute(fox_paged_attn_kernel<kBf16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, PagedTile<D>::kSmem) !=
         cudaSuccess)
       return FOX_ERR_LAUNCH;
+    // (the split of shared memory and L1 as the first kernel has it: changing it needs an SM without CTAs)
+    if (cudaFuncSetAttribute(fox_paged_join_kernel<kBf16, D>, cudaFuncAttributePreferredSharedMemoryCarveout, 100) != cudaSuccess)
+      return FOX_ERR_LAUNCH;
     done.fetch_or(bit, std::memory_order_relaxed);
   }
   if (int rc = launch_behind(fox_paged_attn_kernel<kBf16, D>, dim3(kPagGrid), PagedTile<D>::kThreads, PagedTile<D>::kSmem, st, p, map_k,
                              map_v))
     return rc;
+  if (p.most <= (pag_whole(D) - kPagStart) * kPagTile) return FOX_OK;   // no unit is ever cut between CTAs
   const int64_t pairs = static_cast<int64_t>(p.R) * p.H;
-  return launch_behind(fox_paged_join_kernel<kBf16, D>, dim3((unsigned)(pairs < kSms * 4 ? pairs : kSms * 4)), 256, 0, st, p);
+  return launch_behind(fox_paged_join_kernel<kBf16, D>, dim3((unsigned)(pairs < kSms * 8 ? pairs : kSms * 8)), kJoinThreads, 0, st, p);
 }
 
 }  // namespace fox
@@ -571,7 +721,7 @@ static int64_t paged_rows(int64_t H, int64_t Hk) { return H / Hk < kPagRows ? H 
 
 extern "C" int64_t fox_paged_attn_workspace_floats(int64_t R, int64_t H, int64_t Hk, int64_t D) {
   if (R <= 0 || H <= 0 || Hk <= 0 || D <= 0) return 1;
-  return 2 * (R + 1) + 4 + pag_ranges(D) * 2 * paged_rows(H, Hk) * (D + 4);
+  return R + 1 + 4 + kPagGrid * 2 * (1 + pag_warps(D)) * paged_rows(H, Hk) * (D + 4);
 }
 
 extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t n_pages,
@@ -602,15 +752,20 @@ extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, in
   p.gates = gate_pages; p.g_sp = gp_sp; p.g_sh = gp_sh;
   p.table = block_table; p.table_ld = table_ld; p.lengths = lengths;
   p.o = (uint16_t*)o; p.o_sr = o_sr; p.o_sh = o_sh; p.L = L;
-  p.tiles_before = reinterpret_cast<int64_t*>(workspace);
-  p.part = workspace + (2 * (R + 1) + 3) / 4 * 4;
+  p.before = reinterpret_cast<int*>(workspace);
+  p.part = workspace + (R + 1 + 3) / 4 * 4;
   p.R = (int)R; p.H = (int)H; p.group = (int)(H / Hk); p.rows = (int)paged_rows(H, Hk);
   p.tiles_of_group = (p.group + kPagRows - 1) / kPagRows;
   p.units = (int)Hk * p.tiles_of_group;
+  p.by_units = divisor(p.units);
+  p.by_tiles_of_group = divisor(p.tiles_of_group);
   p.n_pages = (int)n_pages;
   for (p.page_log2 = 4; (int64_t{1} << p.page_log2) < page;) ++p.page_log2;
   p.most = width * page < 2147483647LL - 64 ? width * page : 2147483647LL - 64;
   p.qk_scale = sm_scale * kPagLog2e;
+  // places are counted with 30 bits: so many requests at a time, going by what their table rows could hold
+  const int64_t places = p.units * ((p.most + kPagTile - 1) / kPagTile + kPagStart), at_once = (int64_t{1} << 30) / places;
+  if (at_once < 1) return FOX_ERR_TOO_LARGE;
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf = dtype == FOX_DTYPE_BF16;
   CUtensorMap mk, mv;
@@ -619,10 +774,22 @@ extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, in
   if (!tma_compatible(tk, 2) || !tma_compatible(tv, 2)) return FOX_ERR_ALIGNMENT;
   if (int rc = cached_tmap_4d(&mk, tk, 2, false, bf, 64, kPagTile, true)) return rc;
   if (int rc = cached_tmap_4d(&mv, tv, 2, false, bf, 64, kPagTile, true)) return rc;
-  switch (D) {
-    case 16: return bf ? launch_paged<true, 16>(p, mk, mv, st) : launch_paged<false, 16>(p, mk, mv, st);
-    case 32: return bf ? launch_paged<true, 32>(p, mk, mv, st) : launch_paged<false, 32>(p, mk, mv, st);
-    case 64: return bf ? launch_paged<true, 64>(p, mk, mv, st) : launch_paged<false, 64>(p, mk, mv, st);
-    default: return bf ? launch_paged<true, 128>(p, mk, mv, st) : launch_paged<false, 128>(p, mk, mv, st);
+  auto launch_one = [&] {
+    switch (D) {
+      case 16: return bf ? launch_paged<true, 16>(p, mk, mv, st) : launch_paged<false, 16>(p, mk, mv, st);
+      case 32: return bf ? launch_paged<true, 32>(p, mk, mv, st) : launch_paged<false, 32>(p, mk, mv, st);
+      case 64: return bf ? launch_paged<true, 64>(p, mk, mv, st) : launch_paged<false, 64>(p, mk, mv, st);
+      default: return bf ? launch_paged<true, 128>(p, mk, mv, st) : launch_paged<false, 128>(p, mk, mv, st);
+    }
+  };
+  for (int64_t r0 = 0; r0 < R; r0 += at_once) {
+    p.R = static_cast<int>(R - r0 < at_once ? R - r0 : at_once);
+    if (int rc = launch_one()) return rc;
+    p.q += p.R * q_sr;
+    p.o += p.R * o_sr;
+    p.table += p.R * table_ld;
+    p.lengths += p.R;
+    if (p.L) p.L += p.R * H;
   }
+  return FOX_OK;
 }
