@@ -17,7 +17,7 @@
 // is a running sum (exact where the bias is small, which is where it matters; a prefix sum over the whole request would lose
 // what the cache's length costs), and the parts' sums shift their maxima when they are joined.
 //
-// One lane of a warp asks for a tile (TMA, 128-byte swizzle; the gates of every query head by a copy of 64 bytes) into a ring of
+// One lane of a warp asks for a tile (TMA, 128-byte swizzle; the gates each lane by 16 bytes for itself) into a ring of
 // kStages tiles that is the warp's own: no warp waits for another.  (Each lane copying by cp.async what it feeds to the matrix
 // instructions itself needed no barrier, but its 300 instructions a tile queued for shared memory: 3.6 TB/s.)
 // mma.sync m16n8k16 (the two products are 8 query rows at most; the kernel is bound by memory, with a tensor pipe mostly idle):
@@ -104,6 +104,19 @@ __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, ui
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+// a tile of 64-column halves: (64, rows, halves, heads, pages), innermost first
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* tm, uint64_t* bar, int row, int head, int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %3, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(0), "r"(row), "r"(head), "r"(page)
+      : "memory");
+}
 // four 8 x 8 matrices of 16-bit values, each transposed, one row's address from every lane
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -206,13 +219,23 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   const int total = s_before[kThreads] * p.units, per_cta = pag_per_cta(total), raw = min(static_cast<int>(blockIdx.x) * per_cta, total);   // (148 * per_cta is below 2^30 + 148)
 
   // ---- this CTA's range, moved to the ends of units that are not cut, and in it those of its warps: by one warp, a place to a lane
-  if (warp == 0) {
-    auto find = [&](int t) {   // the unit that place t (< total) of the row belongs to
+  if (warp == 0 && total > 0) {
+    const int raw_end = min(raw + per_cta, total);
+    auto share_of = [&](int t) {   // the last share that begins at or before place t (the same t for all lanes)
       const int q = div_by(p.by_units, t);
-      int lo = 0;   // the last share that begins at or before q
-#pragma unroll
-      for (int s = kThreads / 2; s > 0; s >>= 1)
-        if (s_before[lo + s] <= q) lo += s;
+      constexpr int kStep = kThreads / 32;
+      const int hi = (__popc(__ballot_sync(0xffffffffu, s_before[lane * kStep] <= q)) - 1) * kStep;
+      return hi + __popc(__ballot_sync(0xffffffffu, lane < kStep && s_before[hi + lane] <= q)) - 1;
+    };
+    const int share_lo = share_of(min(raw, total - 1)), share_hi = share_of(min(raw_end, total - 1));
+    auto find = [&](int t) {   // the unit that place t (< total, in these shares) of the row belongs to
+      const int q = div_by(p.by_units, t);
+      int lo = share_lo, hi = share_hi;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_before[mid] <= q) lo = mid;
+        else hi = mid - 1;
+      }
       int before = s_before[lo];
       PagedUnit f;
       f.r = lo * share;
@@ -228,7 +251,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
       f.at = before * p.units + f.unit * f.places;
       return f;
     };
-    int edge = lane ? min(raw + per_cta, total) : raw;   // lane 0: where the range begins; the others: where it ends
+    int edge = lane ? raw_end : raw;   // lane 0: where the range begins; the others: where it ends
     if (edge < total) {
       const PagedUnit f = find(edge);
       if (f.at < edge && f.places <= pag_whole(D)) edge = f.at + f.places;
@@ -244,6 +267,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     }
   }
   __syncthreads();
+  if (total == 0) return;
   const int c_begin = s_range[0], c_end = s_range[1], per = s_range[2];
   if (c_begin >= c_end) return;
   const int t_begin = min(c_begin + warp * per, c_end);
@@ -279,14 +303,16 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   // (rows of gates that no head fills: finite)
 #pragma unroll
   for (int s = 0; s < kStages; ++s) *reinterpret_cast<float4*>(ring_g + s * (Tile::kGates / 4) + lane * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
-  fence_proxy_async_smem();
-  __syncwarp();
+  const uint32_t ring_u32 = smem_u32(ring), gates_u32 = smem_u32(ring_g) + lane * 16;
   int page_r = -1, page_base = 0, page_ids = -1;   // 32 entries of a request's table row, one to a lane
 
   int ask_stage = 0;
   int pending = 0;   // tiles asked for and not yet used
   auto ask = [&]() {   // the next tile
-    if (at < part_lo) return;
+    if (at < part_lo) {
+      cp_async_commit();
+      return;
+    }
     const int key0 = at * kPagTile, j = key0 >> p.page_log2, row0 = key0 & ((1 << p.page_log2) - 1);
     if (r != page_r || j < page_base || j >= page_base + 32) {
       page_r = r;
@@ -300,21 +326,16 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     if (lane == 0) {
       s_item[warp][ask_stage] = {r, h0, there ? min(length - key0, kPagTile) : 0, flags | (last ? kItemLast : 0)};
       if (there) {
-        mbar_expect_tx(bar, Tile::kStage + heads * (kPagTile * 4));
-        char* to = ring + ask_stage * Tile::kStage;
-#pragma unroll
-        for (int s = 0; s < Tile::kHalves; ++s) {
-          tma_load_4d(to + s * Tile::kBox, &map_k, bar, s * 64, row0, kh, id);
-          tma_load_4d(to + (Tile::kHalves + s) * Tile::kBox, &map_v, bar, s * 64, row0, kh, id);
-        }
+        mbar_expect_tx(bar, Tile::kStage);
+        const uint32_t to = ring_u32 + ask_stage * Tile::kStage;
+        tma_load_5d(to, &map_k, bar, row0, kh, id);
+        tma_load_5d(to + Tile::kStage / 2, &map_v, bar, row0, kh, id);
       } else {
         mbar_arrive(bar);
       }
     }
-    __syncwarp();
-    if (there && lane < heads)
-      bulk_load(ring_g + ask_stage * (Tile::kGates / 4) + lane * kPagTile, p.gates + id * p.g_sp + (h0 + lane) * p.g_sh + row0,
-                kPagTile * 4, bar);
+    if (there && x < heads) cp_async_16(gates_u32 + ask_stage * Tile::kGates, p.gates + id * p.g_sp + (h0 + x) * p.g_sh + row0 + 4 * c);
+    cp_async_commit();
     if ((flags & kItemFirst) && x < heads) touch(p.q + r * p.q_sr + (h0 + x) * p.q_sh + (D == 16 ? c * 4 : D == 32 ? c * 8 : c * 16));
     flags &= ~kItemFirst;
     ++pending;
@@ -342,7 +363,6 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   // the row of the values whose address a lane gives: keys 4 (j / 2) + j % 2, in matrices 1 and 3 2 on; in 2 and 3 the next 8 columns
   const uint32_t key_v = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * ((lane >> 3) & 1),
                  v_off = key_v * 128 + ((static_cast<uint32_t>(lane) >> 4) ^ (key_v & 7)) * 16;
-  const uint32_t ring_u32 = smem_u32(ring);
   uint4 qf[2 * Tile::kHalves];   // channels (2 c + s) 8 .. of each half
   float o[Tile::kCols][4], m = -INFINITY, l = 0.f, carry = 0.f;
   int stage = 0;
@@ -352,6 +372,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     if (pending == 0) break;
     if (!mbar_wait_warp(&s_full[warp][stage], parity, &s_abort, p.status, kPagSite, pending)) break;
     --pending;
+    cp_async_wait<kStages - 1>();   // (each lane's own gates)
     __syncwarp();
     const PagedItem item = s_item[warp][stage];
     const uint32_t tile = ring_u32 + stage * Tile::kStage;
@@ -496,6 +517,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
       }
     }
   }
+  cp_async_wait<0>();
   // ---- the parts of this CTA's warps joined: those of the unit that a warp's range begins in, where it ends in that range or the
   // CTA's range ends there, and those of the unit that the CTA's range ends in.  A unit that other CTAs have a part of becomes one
   // part of this CTA's.  The query heads of these units go around the warps.
@@ -690,6 +712,20 @@ __global__ void __launch_bounds__(kJoinThreads) fox_paged_join_kernel(const Page
   }
 }
 
+// (64 columns, rows of a page, halves, heads, pages); a head dim below 64: the columns behind it are filled with zeros
+static int make_paged_tmap(CUtensorMap* out, const fox_tensor4* t, bool bf16, int64_t P, int64_t heads, int64_t page, int64_t D) {
+  EncodeTiledFn fn = get_encode_tiled();
+  if (!fn) return FOX_ERR_DRIVER;
+  const cuuint64_t dims[5] = {(cuuint64_t)(D < 64 ? D : 64), (cuuint64_t)page, (cuuint64_t)(D == 128 ? 2 : 1), (cuuint64_t)heads, (cuuint64_t)P};
+  const cuuint64_t strides[4] = {(cuuint64_t)t->st * 2, 128, (cuuint64_t)t->sh * 2, (cuuint64_t)t->sb * 2};
+  const cuuint32_t box[5] = {64, kPagTile, (cuuint32_t)(D == 128 ? 2 : 1), 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+  return fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, t->ptr, dims, strides, box, ones,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? FOX_OK
+             : FOX_ERR_TENSORMAP;
+}
+
 template <bool kBf16, int D>
 static int launch_paged(const PagedParams& p, const CUtensorMap& map_k, const CUtensorMap& map_v, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};   // devices whose limit has been raised
@@ -769,11 +805,10 @@ extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, in
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf = dtype == FOX_DTYPE_BF16;
   CUtensorMap mk, mv;
-  const Tensor4 tk{k_pages->ptr, n_pages, Hk, page, D, k_pages->sb, k_pages->sh, k_pages->st};
-  const Tensor4 tv{v_pages->ptr, n_pages, Hk, page, D, v_pages->sb, v_pages->sh, v_pages->st};
-  if (!tma_compatible(tk, 2) || !tma_compatible(tv, 2)) return FOX_ERR_ALIGNMENT;
-  if (int rc = cached_tmap_4d(&mk, tk, 2, false, bf, 64, kPagTile, true)) return rc;
-  if (int rc = cached_tmap_4d(&mv, tv, 2, false, bf, 64, kPagTile, true)) return rc;
+  auto bad = [](const fox_tensor4* x) { return x->sb <= 0 || x->sh <= 0 || x->st <= 0; };
+  if (bad(k_pages) || bad(v_pages)) return FOX_ERR_ALIGNMENT;
+  if (int rc = make_paged_tmap(&mk, k_pages, bf, n_pages, Hk, page, D)) return rc;
+  if (int rc = make_paged_tmap(&mv, v_pages, bf, n_pages, Hk, page, D)) return rc;
   auto launch_one = [&] {
     switch (D) {
       case 16: return bf ? launch_paged<true, 16>(p, mk, mv, st) : launch_paged<false, 16>(p, mk, mv, st);
