@@ -70,21 +70,40 @@ __device__ __forceinline__ float rot_weight(const void* w, int dtype, int64_t i)
   const uint32_t u = static_cast<const uint16_t*>(w)[i];
   return dtype == FOX_DTYPE_BF16 ? unpack2<true>(u).x : unpack2<false>(u).x;
 }
+// eight weights from element i on, a multiple of 8 (16-byte aligned)
+__device__ __forceinline__ void rot_weights(const void* w, int dtype, int64_t i, float2* f) {
+  if (dtype == FOX_DTYPE_FP32) {
+    const float4 *v = reinterpret_cast<const float4*>(static_cast<const float*>(w) + i), a = v[0], b = v[1];
+    f[0] = make_float2(a.x, a.y);
+    f[1] = make_float2(a.z, a.w);
+    f[2] = make_float2(b.x, b.y);
+    f[3] = make_float2(b.z, b.w);
+  } else {
+    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + i);
+    if (dtype == FOX_DTYPE_BF16) rot_unpack<true>(v, f);
+    else rot_unpack<false>(v, f);
+  }
+}
 __device__ __forceinline__ float2 rot_mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
 __device__ __forceinline__ float2 rot_fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 rot_both(float a) { return make_float2(a, a); }
 
-// cosines and sines of tokens t0 .. t0 + n of sequence b, (tile, D / 2) each
-__device__ __forceinline__ void rot_angles(const RotaryParams& p, int b, int t0, int n, float* s_cos, float* s_sin) {
+// cosines and sines of tokens t0 .. t0 + n of sequence b, (tile, D / 2) each; s_pos: (tile).  A barrier is inside and one behind.
+__device__ __forceinline__ void rot_angles(const RotaryParams& p, int b, int t0, int n, double* s_pos, float* s_cos, float* s_sin) {
   const int pairs = p.D >> 1;
-  for (int i = threadIdx.x; i < n * p.half; i += blockDim.x) {
-    const int u = div_by(p.by_half, i), f = i - u * p.half, t = t0 + u;
+  for (int u = threadIdx.x; u < n; u += blockDim.x) {
+    const int t = t0 + u;
     int64_t pos = p.first + t * p.step;
     if (p.positions) {
       const int64_t at = b * p.pos_sb + t * p.pos_st;
       pos = p.pos_64 ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
     }
-    const double a = static_cast<double>(pos) * static_cast<double>(p.inv_freq[f]);
+    s_pos[u] = static_cast<double>(pos);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n * p.half; i += blockDim.x) {
+    const int u = div_by(p.by_half, i), f = i - u * p.half;
+    const double a = s_pos[u] * static_cast<double>(p.inv_freq[f]);
     const double turns = rint(a * 0.15915494309189535);
     // less whole turns, 2 pi in two parts; in units of pi
     const double r = fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, a)) * 0.3183098861837907;
@@ -93,6 +112,7 @@ __device__ __forceinline__ void rot_angles(const RotaryParams& p, int b, int t0,
     s_cos[u * pairs + f] = cs * p.scale;
     s_sin[u * pairs + f] = sn * p.scale * p.sign;
   }
+  __syncthreads();
 }
 
 // The rotation of one lane's 8 channels n.  pair: the values half the rotated part away, turned in sign where those are the
@@ -157,7 +177,8 @@ template <bool kBf16, int kMode, bool kNorm>
 __global__ void __launch_bounds__(kRotThreads) fox_rotary_fwd_kernel(const RotaryParams p) {
   extern __shared__ __align__(16) float rot_smem[];
   const int lanes = p.D >> 3, pairs = p.D >> 1;
-  float *s_cos = rot_smem, *s_sin = rot_smem + p.tile * pairs;
+  double* s_pos = reinterpret_cast<double*>(rot_smem);
+  float *s_cos = rot_smem + 2 * kRotTile, *s_sin = s_cos + p.tile * pairs;
   const int sub = threadIdx.x % lanes, slot = threadIdx.x / lanes, head = blockIdx.y * p.heads_here + slot;
   const bool active = slot < p.heads_here && head < p.heads;
   const bool is_k = active && head >= p.H;
@@ -179,18 +200,12 @@ __global__ void __launch_bounds__(kRotThreads) fox_rotary_fwd_kernel(const Rotar
     if (b == static_cast<int>(blockIdx.z) || p.pos_sb) {
       if constexpr (kNorm) {
         if (b == static_cast<int>(blockIdx.z)) {
-          const int64_t at = h * x.w_sh + ch, at_p = at + (from - lane) * 8;
-          auto wv = [&](int64_t i) { return active ? rot_weight(x.w, x.w_dtype, i) : 0.f; };
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            w[j] = make_float2(wv(at + 2 * j), wv(at + 2 * j + 1));
-            if constexpr (kMode == kLanes) wp[j] = make_float2(wv(at_p + 2 * j), wv(at_p + 2 * j + 1));
-          }
+          rot_weights(x.w, x.w_dtype, h * x.w_sh + ch, w);
+          if constexpr (kMode == kLanes) rot_weights(x.w, x.w_dtype, h * x.w_sh + ch + (from - lane) * 8, wp);
         }
       }
       if (b != static_cast<int>(blockIdx.z)) __syncthreads();   // (the last sequence's angles have been used)
-      rot_angles(p, b, t0, n, s_cos, s_sin);
-      __syncthreads();
+      rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
     }
     for (int u0 = 0; u0 < n; u0 += kRotAhead) {
       uint4 raw[kRotAhead];
@@ -215,15 +230,19 @@ __global__ void __launch_bounds__(kRotThreads) fox_rotary_fwd_kernel(const Rotar
           r = rsqrtf(fmaf(ss, inv_d, p.eps));
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            v[j] = rot_mul(v[j], rot_mul(w[j], rot_both(r)));
-            if constexpr (kMode == kLanes) pair[j] = rot_mul(pair[j], rot_mul(wp[j], rot_both(r)));
+            v[j] = rot_mul(v[j], w[j]);
+            if constexpr (kMode == kLanes) pair[j] = rot_mul(pair[j], wp[j]);
           }
         }
         auto other = [&](int d) {
           const float m = active ? rot_weight(row + (u0 + u) * x.x_st - ch, kBf16 ? FOX_DTYPE_BF16 : FOX_DTYPE_FP16, d) : 0.f;
-          return kNorm ? m * (r * (active ? rot_weight(x.w, x.w_dtype, h * x.w_sh + d) : 0.f)) : m;
+          return kNorm ? m * rot_weight(x.w, x.w_dtype, h * x.w_sh + d) : m;
         };
         rot_turn<kMode>(p, ch, s_cos + (u0 + u) * pairs, s_sin + (u0 + u) * pairs, v, pair, other, out);
+        if constexpr (kNorm) {   // (1 / rms last: it is the same for both channels of a pair)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) out[j] = rot_mul(out[j], rot_both(r));
+        }
         if (active) *reinterpret_cast<uint4*>(to + (u0 + u) * x.y_st) = rot_pack<kBf16>(out);
       }
     }
@@ -237,7 +256,8 @@ __global__ void __launch_bounds__(kRotThreads) fox_rotary_bwd_kernel(const Rotar
   constexpr int kAhead = 2;
   extern __shared__ __align__(16) float rot_smem[];
   const int lanes = p.D >> 3, pairs = p.D >> 1;
-  float *s_cos = rot_smem, *s_sin = rot_smem + p.tile * pairs;
+  double* s_pos = reinterpret_cast<double*>(rot_smem);
+  float *s_cos = rot_smem + 2 * kRotTile, *s_sin = s_cos + p.tile * pairs;
   const int sub = threadIdx.x % lanes, slot = threadIdx.x / lanes, head = blockIdx.y * p.heads_here + slot;
   const bool active = slot < p.heads_here && head < p.heads;
   const bool is_k = active && head >= p.H;
@@ -247,12 +267,9 @@ __global__ void __launch_bounds__(kRotThreads) fox_rotary_bwd_kernel(const Rotar
   const uint32_t flip = ch < p.half ? 0x80008000u : 0u;
   wait_for_kernel_in_front();
   float2 w[4], dw[4];
+  rot_weights(x.w, x.w_dtype, h * x.w_sh + ch, w);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t at = h * x.w_sh + ch + 2 * j;
-    w[j] = active ? make_float2(rot_weight(x.w, x.w_dtype, at), rot_weight(x.w, x.w_dtype, at + 1)) : rot_both(0.f);
-    dw[j] = rot_both(0.f);
-  }
+  for (int j = 0; j < 4; ++j) dw[j] = rot_both(0.f);
   const float inv_d = 1.f / static_cast<float>(p.D);
   for (int64_t t64 = static_cast<int64_t>(blockIdx.x) * p.tile; t64 < p.T; t64 += static_cast<int64_t>(gridDim.x) * p.tile) {
     const int t0 = static_cast<int>(t64), n = min(p.tile, p.T - t0);
@@ -271,8 +288,7 @@ __global__ void __launch_bounds__(kRotThreads) fox_rotary_bwd_kernel(const Rotar
       for (int u = 0; u < kAhead; ++u) load(u, ahead_x[u], ahead_g[u]);
       if (b == static_cast<int>(blockIdx.z) || p.pos_sb) {
         __syncthreads();
-        rot_angles(p, b, t0, n, s_cos, s_sin);
-        __syncthreads();
+        rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
       }
       for (int u0 = 0; u0 < n; u0 += kAhead) {
         uint4 raw_x[kAhead], raw_g[kAhead];
@@ -399,7 +415,7 @@ static int rotary_launch(RotaryKind kind, int dtype, int64_t half, int interleav
   p.heads_here = g.heads_here;
   p.tile = g.tile;
   const dim3 grid(g.tiles, g.blocks, g.slices);
-  const size_t smem = static_cast<size_t>(p.tile) * p.D * sizeof(float);
+  const size_t smem = kRotTile * sizeof(double) + static_cast<size_t>(p.tile) * p.D * sizeof(float);
   const bool bf = dtype == FOX_DTYPE_BF16;
   if (interleaved) return bf ? rotary_launch_at<true, kNext>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kNext>(kind, grid, g.threads, smem, st, p);
   if (half % 8) return bf ? rotary_launch_at<true, kAny>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kAny>(kind, grid, g.threads, smem, st, p);
@@ -410,6 +426,7 @@ static bool rotary_bad_rows(const fox_tensor4* t) {
   return reinterpret_cast<uintptr_t>(t->ptr) % 16 || t->sb % 8 || t->sh % 8 || t->st % 8;
 }
 static bool rotary_bad_weight(int dtype) { return dtype != FOX_DTYPE_FP16 && dtype != FOX_DTYPE_BF16 && dtype != FOX_DTYPE_FP32; }
+static bool rotary_bad_weights(const void* w, int64_t sh, int64_t D) { return reinterpret_cast<uintptr_t>(w) % 16 || (sh != 0 && sh != D); }
 
 static int rotary_check(int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D, const float* inv_freq, int64_t half) {
   if (B <= 0 || T <= 0 || H <= 0 || Hk < 0 || half <= 0 || !inv_freq) return FOX_ERR_BAD_ARG;
@@ -476,6 +493,7 @@ extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64
   if (!q || !k || !q_out || !k_out || !q->ptr || !k->ptr || !q_out->ptr || !k_out->ptr || !wq || !wk || Hk <= 0) return FOX_ERR_BAD_ARG;
   if (int rc = rotary_check(dtype, B, T, H, Hk, D, inv_freq, half)) return rc;
   if (rotary_bad_weight(wq_dtype) || rotary_bad_weight(wk_dtype)) return FOX_ERR_BAD_ARG;
+  if (rotary_bad_weights(wq, wq_sh, D) || rotary_bad_weights(wk, wk_sh, D)) return FOX_ERR_ALIGNMENT;
   if (rotary_bad_rows(q) || rotary_bad_rows(k) || rotary_bad_rows(q_out) || rotary_bad_rows(k_out)) return FOX_ERR_ALIGNMENT;
   if (cudaSetDevice(device) != cudaSuccess) return FOX_ERR_DEVICE;
   const bool folded = rotary_fold(B, T);
@@ -505,6 +523,7 @@ extern "C" int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64
     return FOX_ERR_BAD_ARG;
   if (int rc = rotary_check(dtype, B, T, H, Hk, D, inv_freq, half)) return rc;
   if (rotary_bad_weight(wq_dtype) || rotary_bad_weight(wk_dtype)) return FOX_ERR_BAD_ARG;
+  if (rotary_bad_weights(wq, wq_sh, D) || rotary_bad_weights(wk, wk_sh, D)) return FOX_ERR_ALIGNMENT;
   for (const fox_tensor4* t : {q, k, dq_out, dk_out, dq, dk})
     if (rotary_bad_rows(t)) return FOX_ERR_ALIGNMENT;
   if (reinterpret_cast<uintptr_t>(dw_partial) % 16) return FOX_ERR_ALIGNMENT;

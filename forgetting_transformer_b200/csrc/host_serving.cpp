@@ -247,8 +247,11 @@ NormSaved norm_inputs(const Tensor& q, const Tensor& k, const Tensor& wq, const 
     const at::AutoDispatchBelowADInplaceOrView no_autograd;
     a.q = tma_view(q);
     a.k = tma_view(k);
-    a.wq = wq.contiguous();
-    a.wk = wk.contiguous();
+    auto aligned = [](const Tensor& w) {
+      return w.is_contiguous() && reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0 ? w : w.clone(at::MemoryFormat::Contiguous);
+    };
+    a.wq = aligned(wq);
+    a.wk = aligned(wk);
   }
   a.r = std::move(r);
   return a;

@@ -463,7 +463,7 @@ int fox_rotary(int device, void* stream, int dtype, int64_t B, int64_t T, int64_
 
 /* The per-head RMSNorm of q (H heads) and k (Hk heads) and their rotation in one launch (layernorm.py:183-245, rotary.py:22-153;
  * modeling_forgetting_transformer.py:264-265, 314-316).  wq, wk: (heads * D) with stride wq_sh = D, or one (D) for all heads with
- * wq_sh = 0; w*_dtype any FOX_DTYPE_*. */
+ * wq_sh = 0, 16-byte aligned; w*_dtype any FOX_DTYPE_*. */
 int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
                            const fox_tensor4* q, const fox_tensor4* k, const void* wq, int wq_dtype, int64_t wq_sh,
                            const void* wk, int wk_dtype, int64_t wk_sh, float eps, const float* inv_freq, int64_t half,
