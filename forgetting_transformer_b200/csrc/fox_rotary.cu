@@ -13,27 +13,29 @@
 //
 // There is no table of all positions: a CTA forms the angles of its own tile of tokens, once for all of its heads.  The
 // product of position and frequency and its reduction by turns are in 64 bits (at position 10^6 a 32-bit product is off by
-// 0.03 rad), sine and cosine of what is left, at most pi, in 32.
+// 0.03 rad), sine and cosine of what is left, at most pi, by the fast functions in 32.
 //
-// Thread (h, sub) owns the 8 channels [8 sub, 8 sub + 8) of head h (queries' heads, then keys') for every token that its CTA
-// visits: 16-byte loads, the row's sum of squares by a shuffle over D/8 neighbouring lanes, weights and dw in registers.
-// kMode: where the other channel of a pair is:
-//   kNext    in the same lane (neighbouring channels)
-//   kLanes   at the same place of the lane half/8 away (half a multiple of 8): packed values by shuffle
-//   kAny     halves that are no multiple of 8: read from the row again, channel by channel (L1 has it)
+// Thread (h, sub) owns 8 channels of head h (queries' heads, then keys') for every token that its CTA visits; the row's sum of
+// squares is a shuffle over D/8 neighbouring lanes, weights and dw stay in registers.  kMode: which 8 channels, two runs of 4:
+//   kHalves  halves that are a multiple of 4: 4 sub .. of the first half and the same of the second, so that a pair is one
+//            thread's and needs a cosine and a sine once; behind the rotated part 8 channels as they stand.  (With 8 neighbouring
+//            channels a thread and the other ones by shuffle, the kernels were bound by shared memory and shuffles: 66 us
+//            for what takes 48.)
+//   kNext    neighbouring channels paired: 8 neighbouring channels
+//   kAny     halves that are no multiple of 4: 8 neighbouring channels, the others of the pairs read from the row again, one by
+//            one (L1 has it)
 #include "fox_common.cuh"
 #include "fox_host.h"
 
 namespace fox {
 
-enum RotaryMode { kNext, kLanes, kAny };
+enum RotaryMode { kHalves, kNext, kAny };
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTile = 16;      // tokens whose angles are in shared memory at a time
+constexpr int kRotTile = 32;      // tokens whose angles are in shared memory at a time
 constexpr int kRotAhead = 4;      // tokens whose rows a thread has asked for
 constexpr int64_t kRotTokens = (int64_t{1} << 31) - 65536;   // counted with 32 bits, a tile's more among them
-constexpr int kRotFill = kSms * 4;    // CTAs below which tiles are made smaller
-constexpr int kRotShares = kSms * 4;  // CTAs of a backward, each with a share of dw
+constexpr int kRotFwdPerSm = 4, kRotBwdPerSm = 2;   // CTAs, by registers
 
 struct RotaryTensor {
   const uint16_t *x, *dy;
@@ -51,7 +53,7 @@ struct RotaryParams {
   float* dw_partial;              // (shares, heads, D)
   float scale, sign, eps;         // sign: of the sine
   Divisor by_half;
-  int pos_64, half, D, B, T, H, heads, heads_here, tile;
+  int pos_64, half, D, T, tokens, H, heads, heads_here, per_cta, tile;   // per_cta: tokens
 };
 
 template <bool kBf16>
@@ -70,18 +72,54 @@ __device__ __forceinline__ float rot_weight(const void* w, int dtype, int64_t i)
   const uint32_t u = static_cast<const uint16_t*>(w)[i];
   return dtype == FOX_DTYPE_BF16 ? unpack2<true>(u).x : unpack2<false>(u).x;
 }
-// eight weights from element i on, a multiple of 8 (16-byte aligned)
+// four weights from element i on, a multiple of 4 (16-byte aligned in fp32, 8-byte in 16 bits)
 __device__ __forceinline__ void rot_weights(const void* w, int dtype, int64_t i, float2* f) {
   if (dtype == FOX_DTYPE_FP32) {
-    const float4 *v = reinterpret_cast<const float4*>(static_cast<const float*>(w) + i), a = v[0], b = v[1];
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(w) + i);
     f[0] = make_float2(a.x, a.y);
     f[1] = make_float2(a.z, a.w);
-    f[2] = make_float2(b.x, b.y);
-    f[3] = make_float2(b.z, b.w);
   } else {
-    const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(w) + i);
-    if (dtype == FOX_DTYPE_BF16) rot_unpack<true>(v, f);
-    else rot_unpack<false>(v, f);
+    const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(w) + i);
+    f[0] = dtype == FOX_DTYPE_BF16 ? unpack2<true>(v.x) : unpack2<false>(v.x);
+    f[1] = dtype == FOX_DTYPE_BF16 ? unpack2<true>(v.y) : unpack2<false>(v.y);
+  }
+}
+__device__ __forceinline__ uint2 ld_v2_here(const uint16_t* p) {   // (as ld_v4_here)
+  uint2 v;
+  asm volatile("ld.global.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+  return v;
+}
+
+// Where a thread's two runs of 4 channels begin; `turned`: of a rotated part (kHalves).
+struct RotaryRuns {
+  int a, b;
+  bool turned;
+};
+template <int kMode>
+__device__ __forceinline__ RotaryRuns rot_runs(const RotaryParams& p, int sub) {
+  const int quarter = p.half >> 2;   // threads with pairs
+  if (kMode != kHalves || sub >= quarter) {
+    const int ch = kMode != kHalves ? sub * 8 : 2 * p.half + (sub - quarter) * 8;
+    return {ch, ch + 4, kMode != kHalves};
+  }
+  return {4 * sub, p.half + 4 * sub, true};
+}
+template <int kMode>
+__device__ __forceinline__ uint4 rot_load(const uint16_t* row, const RotaryRuns& c) {   // row: of 8 (kHalves: 4) aligned channels
+  if constexpr (kMode == kHalves) {
+    const uint2 a = ld_v2_here(row + c.a), b = ld_v2_here(row + c.b);
+    return make_uint4(a.x, a.y, b.x, b.y);
+  } else {
+    return ld_v4_here(reinterpret_cast<const uint4*>(row + c.a));
+  }
+}
+template <int kMode>
+__device__ __forceinline__ void rot_store(uint16_t* row, const RotaryRuns& c, const uint4& v) {
+  if constexpr (kMode == kHalves) {
+    *reinterpret_cast<uint2*>(row + c.a) = make_uint2(v.x, v.y);
+    *reinterpret_cast<uint2*>(row + c.b) = make_uint2(v.z, v.w);
+  } else {
+    *reinterpret_cast<uint4*>(row + c.a) = v;
   }
 }
 __device__ __forceinline__ float2 rot_mul(float2 a, float2 b) { return __fmul2_rn(a, b); }
@@ -101,28 +139,44 @@ __device__ __forceinline__ void rot_angles(const RotaryParams& p, int b, int t0,
     s_pos[u] = static_cast<double>(pos);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < n * p.half; i += blockDim.x) {
-    const int u = div_by(p.by_half, i), f = i - u * p.half;
-    const double a = s_pos[u] * static_cast<double>(p.inv_freq[f]);
-    const double turns = rint(a * 0.15915494309189535);
-    // less whole turns, 2 pi in two parts; in units of pi
-    const double r = fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, a)) * 0.3183098861837907;
-    float sn, cs;
-    sincospif(static_cast<float>(r), &sn, &cs);
-    s_cos[u * pairs + f] = cs * p.scale;
-    s_sin[u * pairs + f] = sn * p.scale * p.sign;
+  // a thread stays with one frequency (with fewer threads than frequencies, a few)
+  const int across = min(p.half, static_cast<int>(blockDim.x)), groups = div_by(p.by_half, blockDim.x);
+  const int u0 = groups ? div_by(p.by_half, threadIdx.x) : 0, f0 = threadIdx.x - u0 * across;
+  for (int f = u0 < max(groups, 1) ? f0 : p.half; f < p.half; f += across) {
+    const double freq = p.inv_freq[f];
+    for (int u = u0; u < n; u += max(groups, 1)) {
+      const double a = s_pos[u] * freq;
+      const double turns = a * 0.15915494309189535 + 6755399441055744.0 - 6755399441055744.0;   // rounded to whole ones
+      // less whole turns, 2 pi in two parts
+      const float r = static_cast<float>(fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, a)));
+      // (the fast functions: off by 2^-21 at most from minus pi to pi, far below half a step of 16 bits)
+      s_cos[u * pairs + f] = __cosf(r) * p.scale;
+      s_sin[u * pairs + f] = __sinf(r) * (p.scale * p.sign);
+    }
   }
   __syncthreads();
 }
 
-// The rotation of one lane's 8 channels n.  pair: the values half the rotated part away, turned in sign where those are the
-// second ones (kLanes); other(d): the value of channel d (kAny).
+// The rotation of a thread's 8 channels n; other(d): the value of channel d (kAny).
 template <int kMode, class Other>
-__device__ __forceinline__ void rot_turn(const RotaryParams& p, int ch, const float* c, const float* s, const float2* n,
-                                         const float2* pair, Other&& other, float2* out) {
-  if constexpr (kMode == kNext) {
-    if (ch + 8 <= 2 * p.half) {
-      const float4 cs = *reinterpret_cast<const float4*>(c + (ch >> 1)), sn = *reinterpret_cast<const float4*>(s + (ch >> 1));
+__device__ __forceinline__ void rot_turn(const RotaryParams& p, const RotaryRuns& at, const float* c, const float* s, const float2* n,
+                                         Other&& other, float2* out) {
+  if constexpr (kMode == kHalves) {
+    if (at.turned) {
+      const float4 cv = *reinterpret_cast<const float4*>(c + at.a), sv = *reinterpret_cast<const float4*>(s + at.a);
+      const float2 c0 = make_float2(cv.x, cv.y), c1 = make_float2(cv.z, cv.w), s0 = make_float2(sv.x, sv.y), s1 = make_float2(sv.z, sv.w);
+      const float2 m0 = make_float2(-s0.x, -s0.y), m1 = make_float2(-s1.x, -s1.y);
+      out[0] = rot_fma(n[0], c0, rot_mul(n[2], m0));
+      out[1] = rot_fma(n[1], c1, rot_mul(n[3], m1));
+      out[2] = rot_fma(n[2], c0, rot_mul(n[0], s0));
+      out[3] = rot_fma(n[3], c1, rot_mul(n[1], s1));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) out[j] = n[j];
+    }
+  } else if constexpr (kMode == kNext) {
+    if (at.a + 8 <= 2 * p.half) {
+      const float4 cs = *reinterpret_cast<const float4*>(c + (at.a >> 1)), sn = *reinterpret_cast<const float4*>(s + (at.a >> 1));
       const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j)
@@ -130,23 +184,10 @@ __device__ __forceinline__ void rot_turn(const RotaryParams& p, int ch, const fl
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int i = (ch >> 1) + j;
+        const int i = (at.a >> 1) + j;
         const float cv = i < p.half ? c[i] : 1.f, sv = i < p.half ? s[i] : 0.f;
         out[j] = make_float2(n[j].x * cv - n[j].y * sv, n[j].y * cv + n[j].x * sv);
       }
-    }
-  } else if constexpr (kMode == kLanes) {
-    if (ch < 2 * p.half) {
-      const int i0 = ch < p.half ? ch : ch - p.half;
-      const float4 c0 = *reinterpret_cast<const float4*>(c + i0), c1 = *reinterpret_cast<const float4*>(c + i0 + 4);
-      const float4 s0 = *reinterpret_cast<const float4*>(s + i0), s1 = *reinterpret_cast<const float4*>(s + i0 + 4);
-      out[0] = rot_fma(n[0], make_float2(c0.x, c0.y), rot_mul(pair[0], make_float2(s0.x, s0.y)));
-      out[1] = rot_fma(n[1], make_float2(c0.z, c0.w), rot_mul(pair[1], make_float2(s0.z, s0.w)));
-      out[2] = rot_fma(n[2], make_float2(c1.x, c1.y), rot_mul(pair[2], make_float2(s1.x, s1.y)));
-      out[3] = rot_fma(n[3], make_float2(c1.z, c1.w), rot_mul(pair[3], make_float2(s1.z, s1.w)));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) out[j] = n[j];
     }
   } else {
     auto one = [&](int d, float v) {
@@ -157,158 +198,157 @@ __device__ __forceinline__ void rot_turn(const RotaryParams& p, int ch, const fl
       return v * c[i] + m * (low ? -s[i] : s[i]);
     };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = make_float2(one(ch + 2 * j, n[j].x), one(ch + 2 * j + 1, n[j].y));
+    for (int j = 0; j < 4; ++j) out[j] = make_float2(one(at.a + 2 * j, n[j].x), one(at.a + 2 * j + 1, n[j].y));
   }
 }
 
-// lane of the other channels of a pair, for kLanes (a lane beyond the rotated part: itself)
-__device__ __forceinline__ int rot_partner(const RotaryParams& p, int ch, int lane) {
-  return ch < p.half ? lane + (p.half >> 3) : ch < 2 * p.half ? lane - (p.half >> 3) : lane;
-}
-// the packed values of another lane, `flip` (both sign bits, or none) turned
-__device__ __forceinline__ uint4 rot_shuffle(const uint4& v, int from, uint32_t flip) {
-  return make_uint4(__shfl_sync(0xffffffffu, v.x, from) ^ flip, __shfl_sync(0xffffffffu, v.y, from) ^ flip,
-                    __shfl_sync(0xffffffffu, v.z, from) ^ flip, __shfl_sync(0xffffffffu, v.w, from) ^ flip);
-}
-
-// grid: (tiles of a sequence's tokens, blocks of heads_here heads, every which sequence); blockDim.x = heads_here * D / 8 up to a
-// whole warp.  Positions that all sequences share: their angles are formed once for all sequences of a CTA.
-template <bool kBf16, int kMode, bool kNorm>
-__global__ void __launch_bounds__(kRotThreads) fox_rotary_fwd_kernel(const RotaryParams p) {
+// grid: (ranges of per_cta tokens, blocks of heads_here heads); blockDim.x = heads_here * D / 8 up to a whole warp.  One wave of
+// CTAs with equal ranges, each in tiles of one sequence's tokens: of tiles as CTAs (16 tokens, 2.3 waves of them) the
+// norm of 2 x 8192 tokens x 32 heads of 128 took 74 us.
+template <bool kBf16, int kMode, bool kNorm, int kD>
+__global__ void __launch_bounds__(kRotThreads, kRotFwdPerSm) fox_rotary_fwd_kernel(const RotaryParams p) {
   extern __shared__ __align__(16) float rot_smem[];
-  const int lanes = p.D >> 3, pairs = p.D >> 1;
+  const int D = kD ? kD : p.D, lanes = D >> 3, pairs = D >> 1;
   double* s_pos = reinterpret_cast<double*>(rot_smem);
   float *s_cos = rot_smem + 2 * kRotTile, *s_sin = s_cos + p.tile * pairs;
   const int sub = threadIdx.x % lanes, slot = threadIdx.x / lanes, head = blockIdx.y * p.heads_here + slot;
   const bool active = slot < p.heads_here && head < p.heads;
   const bool is_k = active && head >= p.H;
   const RotaryTensor& x = p.t[is_k];
-  const int h = active ? (is_k ? head - p.H : head) : 0, ch = sub * 8;
-  const int lane = threadIdx.x & 31, from = rot_partner(p, ch, lane);
-  const uint32_t flip = ch < p.half ? 0x80008000u : 0u;
-  const int t0 = blockIdx.x * p.tile, n = min(p.tile, p.T - t0);
+  const int h = active ? (is_k ? head - p.H : head) : 0;
+  const RotaryRuns ch = rot_runs<kMode>(p, sub);
   wait_for_kernel_in_front();
-  float2 w[4], wp[4];
-  const float inv_d = 1.f / static_cast<float>(p.D);
-  for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
-    const uint16_t* row = x.x + b * x.x_sb + h * x.x_sh + t0 * x.x_st + ch;
-    uint16_t* to = x.y + b * x.y_sb + h * x.y_sh + t0 * x.y_st + ch;
-    auto load = [&](int u) { return active && u < n ? ld_v4_here(reinterpret_cast<const uint4*>(row + u * x.x_st)) : make_uint4(0, 0, 0, 0); };
+  const int begin = static_cast<int>(blockIdx.x) * p.per_cta, end = min(begin + p.per_cta, p.tokens);
+  float2 w[4];
+  const int64_t x_st = x.x_st, y_st = x.y_st;
+  const float inv_d = 1.f / static_cast<float>(D);
+  for (int at = begin, n; at < end; at += n) {
+    const int b = at / p.T, t0 = at - b * p.T;
+    n = min(min(p.tile, end - at), p.T - t0);
+    const uint16_t* row = x.x + b * x.x_sb + h * x.x_sh + t0 * x.x_st;
+    uint16_t* to = x.y + b * x.y_sb + h * x.y_sh + t0 * x.y_st;
+    int to_ask = active ? n : 0;
     uint4 ahead[kRotAhead];
+    auto ask = [&] {
 #pragma unroll
-    for (int u = 0; u < kRotAhead; ++u) ahead[u] = load(u);
-    if (b == static_cast<int>(blockIdx.z) || p.pos_sb) {
-      if constexpr (kNorm) {
-        if (b == static_cast<int>(blockIdx.z)) {
-          rot_weights(x.w, x.w_dtype, h * x.w_sh + ch, w);
-          if constexpr (kMode == kLanes) rot_weights(x.w, x.w_dtype, h * x.w_sh + ch + (from - lane) * 8, wp);
-        }
+      for (int u = 0; u < kRotAhead; ++u) ahead[u] = u < to_ask ? rot_load<kMode>(row + u * x_st, ch) : make_uint4(0, 0, 0, 0);
+      row += kRotAhead * x_st;
+      to_ask -= kRotAhead;
+    };
+    ask();
+    if constexpr (kNorm) {
+      if (at == begin) {
+        rot_weights(x.w, x.w_dtype, h * x.w_sh + ch.a, w);
+        rot_weights(x.w, x.w_dtype, h * x.w_sh + ch.b, w + 2);
       }
-      if (b != static_cast<int>(blockIdx.z)) __syncthreads();   // (the last sequence's angles have been used)
-      rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
     }
-    for (int u0 = 0; u0 < n; u0 += kRotAhead) {
+    if (at != begin) __syncthreads();   // (the last tile's angles have been used)
+    rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
+    const float *c = s_cos, *s = s_sin;
+    for (int left = n; left > 0; left -= kRotAhead) {
       uint4 raw[kRotAhead];
 #pragma unroll
-      for (int u = 0; u < kRotAhead; ++u) {
-        raw[u] = ahead[u];
-        ahead[u] = load(u0 + kRotAhead + u);
-      }
+      for (int u = 0; u < kRotAhead; ++u) raw[u] = ahead[u];
+      ask();
 #pragma unroll
       for (int u = 0; u < kRotAhead; ++u) {
-        if (u0 + u >= n) break;   // (the same for all threads)
-        float2 v[4], pair[4], out[4];
+        if (u >= left) break;   // (the same for all threads)
+        float2 v[4], out[4];
         float r = 1.f;
         rot_unpack<kBf16>(raw[u], v);
-        if constexpr (kMode == kLanes) rot_unpack<kBf16>(rot_shuffle(raw[u], from, flip), pair);
         if constexpr (kNorm) {
           float2 sq = rot_mul(v[0], v[0]);
 #pragma unroll
           for (int j = 1; j < 4; ++j) sq = rot_fma(v[j], v[j], sq);
           float ss = sq.x + sq.y;
+#pragma unroll
           for (int o = lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
           r = rsqrtf(fmaf(ss, inv_d, p.eps));
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v[j] = rot_mul(v[j], w[j]);
-            if constexpr (kMode == kLanes) pair[j] = rot_mul(pair[j], wp[j]);
-          }
+          for (int j = 0; j < 4; ++j) v[j] = rot_mul(v[j], w[j]);
         }
-        auto other = [&](int d) {
-          const float m = active ? rot_weight(row + (u0 + u) * x.x_st - ch, kBf16 ? FOX_DTYPE_BF16 : FOX_DTYPE_FP16, d) : 0.f;
+        auto other = [&](int d) {   // (row is two batches on)
+          const float m = active ? rot_weight(row + (u - 2 * kRotAhead) * x_st, kBf16 ? FOX_DTYPE_BF16 : FOX_DTYPE_FP16, d) : 0.f;
           return kNorm ? m * rot_weight(x.w, x.w_dtype, h * x.w_sh + d) : m;
         };
-        rot_turn<kMode>(p, ch, s_cos + (u0 + u) * pairs, s_sin + (u0 + u) * pairs, v, pair, other, out);
+        rot_turn<kMode>(p, ch, c + u * pairs, s + u * pairs, v, other, out);
         if constexpr (kNorm) {   // (1 / rms last: it is the same for both channels of a pair)
 #pragma unroll
           for (int j = 0; j < 4; ++j) out[j] = rot_mul(out[j], rot_both(r));
         }
-        if (active) *reinterpret_cast<uint4*>(to + (u0 + u) * x.y_st) = rot_pack<kBf16>(out);
+        if (active) rot_store<kMode>(to + u * y_st, ch, rot_pack<kBf16>(out));
       }
+      to += kRotAhead * y_st;
+      c += kRotAhead * pairs;
+      s += kRotAhead * pairs;
     }
   }
 }
 
-// The norm's backward with the rotation in front.  A CTA takes every grid.x-th tile of every grid.z-th sequence, so that its share
-// of dw stays in registers; fox_rotary_dw_kernel adds the shares in a fixed order.
-template <bool kBf16, int kMode>
-__global__ void __launch_bounds__(kRotThreads) fox_rotary_bwd_kernel(const RotaryParams p) {
+// The norm's backward with the rotation in front.  A CTA's share of dw stays in registers; fox_rotary_dw_kernel adds the
+// shares in a fixed order.
+template <bool kBf16, int kMode, int kD>
+__global__ void __launch_bounds__(kRotThreads, kRotBwdPerSm) fox_rotary_bwd_kernel(const RotaryParams p) {
   constexpr int kAhead = 2;
   extern __shared__ __align__(16) float rot_smem[];
-  const int lanes = p.D >> 3, pairs = p.D >> 1;
+  const int D = kD ? kD : p.D, lanes = D >> 3, pairs = D >> 1;
   double* s_pos = reinterpret_cast<double*>(rot_smem);
   float *s_cos = rot_smem + 2 * kRotTile, *s_sin = s_cos + p.tile * pairs;
   const int sub = threadIdx.x % lanes, slot = threadIdx.x / lanes, head = blockIdx.y * p.heads_here + slot;
   const bool active = slot < p.heads_here && head < p.heads;
   const bool is_k = active && head >= p.H;
   const RotaryTensor& x = p.t[is_k];
-  const int h = active ? (is_k ? head - p.H : head) : 0, ch = sub * 8;
-  const int lane = threadIdx.x & 31, from = rot_partner(p, ch, lane);
-  const uint32_t flip = ch < p.half ? 0x80008000u : 0u;
+  const int h = active ? (is_k ? head - p.H : head) : 0;
+  const RotaryRuns ch = rot_runs<kMode>(p, sub);
   wait_for_kernel_in_front();
   float2 w[4], dw[4];
-  rot_weights(x.w, x.w_dtype, h * x.w_sh + ch, w);
+  rot_weights(x.w, x.w_dtype, h * x.w_sh + ch.a, w);
+  rot_weights(x.w, x.w_dtype, h * x.w_sh + ch.b, w + 2);
 #pragma unroll
   for (int j = 0; j < 4; ++j) dw[j] = rot_both(0.f);
-  const float inv_d = 1.f / static_cast<float>(p.D);
-  for (int64_t t64 = static_cast<int64_t>(blockIdx.x) * p.tile; t64 < p.T; t64 += static_cast<int64_t>(gridDim.x) * p.tile) {
-    const int t0 = static_cast<int>(t64), n = min(p.tile, p.T - t0);
-    for (int b = blockIdx.z; b < p.B; b += gridDim.z) {
-      const uint16_t *row = x.x + b * x.x_sb + h * x.x_sh + t0 * x.x_st + ch, *row_g = x.dy + b * x.dy_sb + h * x.dy_sh + t0 * x.dy_st + ch;
-      uint16_t* to = x.y + b * x.y_sb + h * x.y_sh + t0 * x.y_st + ch;
+  const int64_t x_st = x.x_st, dy_st = x.dy_st, y_st = x.y_st;
+  const float inv_d = 1.f / static_cast<float>(D);
+  const int begin = static_cast<int>(blockIdx.x) * p.per_cta, end = min(begin + p.per_cta, p.tokens);
+  for (int at = begin, n; at < end; at += n) {
+    const int b = at / p.T, t0 = at - b * p.T;
+    n = min(min(p.tile, end - at), p.T - t0);
+    {
+      const uint16_t *row = x.x + b * x.x_sb + h * x.x_sh + t0 * x.x_st, *row_g = x.dy + b * x.dy_sb + h * x.dy_sh + t0 * x.dy_st;
+      uint16_t* to = x.y + b * x.y_sb + h * x.y_sh + t0 * x.y_st;
       uint4 ahead_x[kAhead], ahead_g[kAhead];
-      auto load = [&](int u, uint4& vx, uint4& vg) {
-        vx = vg = make_uint4(0, 0, 0, 0);
-        if (active && u < n) {
-          vx = ld_v4_here(reinterpret_cast<const uint4*>(row + u * x.x_st));
-          vg = ld_v4_here(reinterpret_cast<const uint4*>(row_g + u * x.dy_st));
-        }
-      };
+      int to_ask = active ? n : 0;
+      auto ask = [&] {
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) load(u, ahead_x[u], ahead_g[u]);
-      if (b == static_cast<int>(blockIdx.z) || p.pos_sb) {
-        __syncthreads();
-        rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
-      }
-      for (int u0 = 0; u0 < n; u0 += kAhead) {
+        for (int u = 0; u < kAhead; ++u) {
+          ahead_x[u] = u < to_ask ? rot_load<kMode>(row + u * x_st, ch) : make_uint4(0, 0, 0, 0);
+          ahead_g[u] = u < to_ask ? rot_load<kMode>(row_g + u * dy_st, ch) : make_uint4(0, 0, 0, 0);
+        }
+        row += kAhead * x_st;
+        row_g += kAhead * dy_st;
+        to_ask -= kAhead;
+      };
+      ask();
+      if (at != begin) __syncthreads();   // (the last tile's angles have been used)
+      rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
+      const float *c = s_cos, *s = s_sin;
+      for (int left = n; left > 0; left -= kAhead) {
         uint4 raw_x[kAhead], raw_g[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           raw_x[u] = ahead_x[u];
           raw_g[u] = ahead_g[u];
-          load(u0 + kAhead + u, ahead_x[u], ahead_g[u]);
         }
+        ask();
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          if (u0 + u >= n) break;
-          float2 v[4], g[4], pair[4], dn[4], gw[4], out[4];
+          if (u >= left) break;
+          float2 v[4], g[4], dn[4], gw[4], out[4];
           rot_unpack<kBf16>(raw_x[u], v);
           rot_unpack<kBf16>(raw_g[u], g);
-          if constexpr (kMode == kLanes) rot_unpack<kBf16>(rot_shuffle(raw_g[u], from, flip), pair);
-          auto other = [&](int d) {
-            return active ? rot_weight(row_g + (u0 + u) * x.dy_st - ch, kBf16 ? FOX_DTYPE_BF16 : FOX_DTYPE_FP16, d) : 0.f;
+          auto other = [&](int d) {   // (row_g is two batches on)
+            return active ? rot_weight(row_g + (u - 2 * kAhead) * dy_st, kBf16 ? FOX_DTYPE_BF16 : FOX_DTYPE_FP16, d) : 0.f;
           };
-          rot_turn<kMode>(p, ch, s_cos + (u0 + u) * pairs, s_sin + (u0 + u) * pairs, g, pair, other, dn);
+          rot_turn<kMode>(p, ch, c + u * pairs, s + u * pairs, g, other, dn);
           float2 sq = rot_both(0.f), dot2 = rot_both(0.f);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -317,6 +357,7 @@ __global__ void __launch_bounds__(kRotThreads) fox_rotary_bwd_kernel(const Rotar
             dot2 = rot_fma(gw[j], v[j], dot2);
           }
           float ss = sq.x + sq.y, dot = dot2.x + dot2.y;
+#pragma unroll
           for (int o = lanes >> 1; o > 0; o >>= 1) {
             ss += __shfl_xor_sync(0xffffffffu, ss, o);
             dot += __shfl_xor_sync(0xffffffffu, dot, o);
@@ -329,16 +370,18 @@ __global__ void __launch_bounds__(kRotThreads) fox_rotary_bwd_kernel(const Rotar
             dw[j] = rot_fma(dn[j], xhat, dw[j]);
             out[j] = rot_fma(xhat, back, rot_mul(gw[j], r2));
           }
-          if (active) *reinterpret_cast<uint4*>(to + (u0 + u) * x.y_st) = rot_pack<kBf16>(out);
+          if (active) rot_store<kMode>(to + u * y_st, ch, rot_pack<kBf16>(out));
         }
+        to += kAhead * y_st;
+        c += kAhead * pairs;
+        s += kAhead * pairs;
       }
     }
   }
   if (active) {
-    const int64_t share = static_cast<int64_t>(blockIdx.z) * gridDim.x + blockIdx.x;
-    float* to = p.dw_partial + (share * p.heads + head) * p.D + ch;
-    reinterpret_cast<float4*>(to)[0] = make_float4(dw[0].x, dw[0].y, dw[1].x, dw[1].y);
-    reinterpret_cast<float4*>(to)[1] = make_float4(dw[2].x, dw[2].y, dw[3].x, dw[3].y);
+    float* to = p.dw_partial + (static_cast<int64_t>(blockIdx.x) * p.heads + head) * p.D;
+    *reinterpret_cast<float4*>(to + ch.a) = make_float4(dw[0].x, dw[0].y, dw[1].x, dw[1].y);
+    *reinterpret_cast<float4*>(to + ch.b) = make_float4(dw[2].x, dw[2].y, dw[3].x, dw[3].y);
   }
 }
 
@@ -382,44 +425,42 @@ __global__ void __launch_bounds__(256) fox_rotary_dw_kernel(const RotaryDwParams
 
 // ------------------------------------------------------------------- launches
 struct RotaryGrid {
-  int blocks, heads_here, threads, tile, tiles, slices;   // slices: of the sequences
+  int blocks, heads_here, threads, ranges, per_cta, tile;
 };
-// Heads of a token over as few CTAs of up to 256 threads as hold them, evenly.  Tiles of 16 tokens, and smaller ones where those of
-// all sequences do not fill the GPU; as few slices of the sequences as do, so that angles are formed once for several.
-static RotaryGrid rotary_grid(int64_t heads, int64_t D, int64_t B, int64_t T) {
+// Heads of a token over as few CTAs of up to 256 threads as hold them, evenly; tokens over as many ranges as make one wave.
+static RotaryGrid rotary_grid(int64_t heads, int64_t D, int64_t tokens, int per_sm) {
   const int64_t most = kRotThreads / (D / 8), blocks = (heads + most - 1) / most, here = (heads + blocks - 1) / blocks;
-  const int64_t fit = (T * B * blocks + kRotFill - 1) / kRotFill, tile = fit < 1 ? 1 : fit < kRotTile ? fit : kRotTile;
-  const int64_t tiles = (T + tile - 1) / tile, want = (2 * kRotFill + tiles * blocks - 1) / (tiles * blocks);
-  const int64_t slices = want < B ? want : B;
-  return {static_cast<int>(blocks), static_cast<int>(here), static_cast<int>((here * (D / 8) + 31) / 32 * 32), static_cast<int>(tile),
-          static_cast<int>(tiles), static_cast<int>(slices < 65535 ? slices : 65535)};
-}
-// A backward's CTAs to a block of heads: (tiles, slices), with some kRotShares CTAs in all.
-static RotaryGrid rotary_grid_bwd(int64_t heads, int64_t D, int64_t B, int64_t T) {
-  RotaryGrid g = rotary_grid(heads, D, B, T);
-  const int most = (kRotShares + g.blocks - 1) / g.blocks;
-  if (g.tiles > most) g.tiles = most;
-  const int want = most / g.tiles;
-  g.slices = static_cast<int>(want < B ? want : B);
-  return g;
+  const int64_t fit = kSms * per_sm / blocks, want = fit < 1 ? 1 : fit, per = (tokens + want - 1) / want;
+  return {static_cast<int>(blocks), static_cast<int>(here), static_cast<int>((here * (D / 8) + 31) / 32 * 32),
+          static_cast<int>((tokens + per - 1) / per), static_cast<int>(per), static_cast<int>(per < kRotTile ? per : kRotTile)};
 }
 
 enum RotaryKind { kTurn, kNormTurn, kNormBack };
+template <bool kBf16, int kMode, int kD>
+static int rotary_launch_of(RotaryKind kind, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const RotaryParams& p) {
+  if (kind == kTurn) return launch_behind(fox_rotary_fwd_kernel<kBf16, kMode, false, kD>, grid, threads, smem, st, p);
+  if (kind == kNormTurn) return launch_behind(fox_rotary_fwd_kernel<kBf16, kMode, true, kD>, grid, threads, smem, st, p);
+  return launch_behind(fox_rotary_bwd_kernel<kBf16, kMode, kD>, grid, threads, smem, st, p);
+}
+// (the head dims of the layers' own configurations as constants; others, and halves that are no multiple of 4, by the general kernel)
 template <bool kBf16, int kMode>
 static int rotary_launch_at(RotaryKind kind, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const RotaryParams& p) {
-  if (kind == kTurn) return launch_behind(fox_rotary_fwd_kernel<kBf16, kMode, false>, grid, threads, smem, st, p);
-  if (kind == kNormTurn) return launch_behind(fox_rotary_fwd_kernel<kBf16, kMode, true>, grid, threads, smem, st, p);
-  return launch_behind(fox_rotary_bwd_kernel<kBf16, kMode>, grid, threads, smem, st, p);
+  if constexpr (kMode != kAny) {
+    if (p.D == 64) return rotary_launch_of<kBf16, kMode, 64>(kind, grid, threads, smem, st, p);
+    if (p.D == 128) return rotary_launch_of<kBf16, kMode, 128>(kind, grid, threads, smem, st, p);
+  }
+  return rotary_launch_of<kBf16, kMode, 0>(kind, grid, threads, smem, st, p);
 }
 static int rotary_launch(RotaryKind kind, int dtype, int64_t half, int interleaved, const RotaryGrid& g, cudaStream_t st, RotaryParams p) {
   p.heads_here = g.heads_here;
   p.tile = g.tile;
-  const dim3 grid(g.tiles, g.blocks, g.slices);
+  p.per_cta = g.per_cta;
+  const dim3 grid(g.ranges, g.blocks);
   const size_t smem = kRotTile * sizeof(double) + static_cast<size_t>(p.tile) * p.D * sizeof(float);
   const bool bf = dtype == FOX_DTYPE_BF16;
   if (interleaved) return bf ? rotary_launch_at<true, kNext>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kNext>(kind, grid, g.threads, smem, st, p);
-  if (half % 8) return bf ? rotary_launch_at<true, kAny>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kAny>(kind, grid, g.threads, smem, st, p);
-  return bf ? rotary_launch_at<true, kLanes>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kLanes>(kind, grid, g.threads, smem, st, p);
+  if (half % 4) return bf ? rotary_launch_at<true, kAny>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kAny>(kind, grid, g.threads, smem, st, p);
+  return bf ? rotary_launch_at<true, kHalves>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kHalves>(kind, grid, g.threads, smem, st, p);
 }
 
 static bool rotary_bad_rows(const fox_tensor4* t) {
@@ -455,7 +496,7 @@ static RotaryParams rotary_params(int64_t B, int64_t T, int64_t H, int64_t Hk, i
   p.first = first; p.step = folded ? 0 : 1; p.pos_64 = pos_64;
   p.scale = scale; p.sign = 1.f; p.eps = eps;
   p.by_half = divisor(half);
-  p.half = (int)half; p.D = (int)D; p.B = (int)B; p.T = (int)T;
+  p.half = (int)half; p.D = (int)D; p.T = (int)T; p.tokens = (int)(B * T);
   p.H = (int)H; p.heads = (int)(H + Hk);
   return p;
 }
@@ -482,7 +523,7 @@ extern "C" int fox_rotary(int device, void* stream, int dtype, int64_t B, int64_
   p.sign = inverse ? -1.f : 1.f;
   rotary_in(p.t[0], rotary_view(x, folded));
   rotary_out(p.t[0], rotary_view(y, folded));
-  return rotary_launch(kTurn, dtype, half, interleaved, rotary_grid(H, D, B, T), (cudaStream_t)stream, p);
+  return rotary_launch(kTurn, dtype, half, interleaved, rotary_grid(H, D, B * T, kRotFwdPerSm), (cudaStream_t)stream, p);
 }
 
 extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
@@ -502,14 +543,12 @@ extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64
   rotary_out(p.t[0], rotary_view(q_out, folded)); rotary_out(p.t[1], rotary_view(k_out, folded));
   p.t[0].w = wq; p.t[0].w_dtype = wq_dtype; p.t[0].w_sh = wq_sh;
   p.t[1].w = wk; p.t[1].w_dtype = wk_dtype; p.t[1].w_sh = wk_sh;
-  return rotary_launch(kNormTurn, dtype, half, interleaved, rotary_grid(H + Hk, D, B, T), (cudaStream_t)stream, p);
+  return rotary_launch(kNormTurn, dtype, half, interleaved, rotary_grid(H + Hk, D, B * T, kRotFwdPerSm), (cudaStream_t)stream, p);
 }
 
 extern "C" int64_t fox_qk_norm_rotary_partials(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D) {
   if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || (D != 16 && D != 32 && D != 64 && D != 128)) return 1;
-  rotary_fold(B, T);
-  const RotaryGrid g = rotary_grid_bwd(H + Hk, D, B, T);
-  return static_cast<int64_t>(g.tiles) * g.slices;
+  return rotary_grid(H + Hk, D, B * T, kRotBwdPerSm).ranges;
 }
 
 extern "C" int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
@@ -542,11 +581,10 @@ extern "C" int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64
   p.t[0].w = wq; p.t[0].w_dtype = wq_dtype; p.t[0].w_sh = wq_sh;
   p.t[1].w = wk; p.t[1].w_dtype = wk_dtype; p.t[1].w_sh = wk_sh;
   p.dw_partial = dw_partial;
-  const RotaryGrid g = rotary_grid_bwd(H + Hk, D, B, T);
-  const int64_t n = static_cast<int64_t>(g.tiles) * g.slices;
+  const RotaryGrid g = rotary_grid(H + Hk, D, B * T, kRotBwdPerSm);
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = rotary_launch(kNormBack, dtype, half, interleaved, g, st, p)) return rc;
-  const RotaryDwParams d{dw_partial, {dwq, dwk}, {wq_dtype, wk_dtype}, {wq_sh == 0, wk_sh == 0}, {(int)H, (int)Hk}, (int)n, (int)D};
+  const RotaryDwParams d{dw_partial, {dwq, dwk}, {wq_dtype, wk_dtype}, {wq_sh == 0, wk_sh == 0}, {(int)H, (int)Hk}, g.ranges, (int)D};
   const int64_t cols = (wq_sh ? H * D : D) + (wk_sh ? Hk * D : D);
   return launch_behind(fox_rotary_dw_kernel, dim3((unsigned)(cols / 16)), 256, 0, st, d);
 }
