@@ -47,27 +47,34 @@ struct TableParams {
 
 __device__ __forceinline__ int clamp31(int64_t x) { return x > 2147483647LL ? 2147483647 : static_cast<int>(x); }
 
+// What a token is placed by, for every request: first token of the packed batch, tokens granted, old length, pages taken by the
+// requests in front.  (starts has one more; free_before: pages that were free.)
+struct Placing {
+  const int32_t *starts, *granted, *lengths, *taken;   // lengths: with what was granted
+  int free_before;
+};
+
 // Token t's request, position and slot.  A page that the call has given out is known from the stack, without the table; the
 // token at its first place writes the table's entry (there is one: a fresh page begins at or behind the old length).
-__device__ __forceinline__ void place_token(const TableParams& p, int t) {
+__device__ __forceinline__ void place_token(const TableParams& p, const Placing& a, int t) {
   int lo = 0, hi = p.R;   // the last request that starts at or before t, so that t < starts[lo + 1] where there is one
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (p.starts[mid] <= t) lo = mid;
+    if (a.starts[mid] <= t) lo = mid;
     else hi = mid;
   }
   int request = -1, pos = 0, slot = -1;
-  if (t < p.starts[p.R]) {
+  if (t < a.starts[p.R]) {
     request = lo;
-    const int n = p.granted[lo], old = p.lengths_out[lo] - n;
-    const int64_t at = static_cast<int64_t>(old) + t - p.starts[lo];
+    const int n = a.granted[lo], old = a.lengths[lo] - n;
+    const int64_t at = static_cast<int64_t>(old) + t - a.starts[lo];
     pos = clamp31(at);
     if (n > 0) {
       const int j = pos >> p.page_log2, have = static_cast<int>((static_cast<int64_t>(old) + (1 << p.page_log2) - 1) >> p.page_log2);
       int32_t* entry = p.table + lo * p.table_ld + j;
       int id;
       if (j >= have) {
-        id = p.free_pages[p.work[p.R] - 1 - (p.work[lo] + j - have)];
+        id = p.free_pages[a.free_before - 1 - (a.taken[lo] + j - have)];
         if ((pos & ((1 << p.page_log2) - 1)) == 0) *entry = id;
       } else {
         id = *entry;
@@ -85,10 +92,14 @@ __device__ __forceinline__ void place_token(const TableParams& p, int t) {
 // the free pages) gets nothing and keeps its length.
 __global__ void __launch_bounds__(kTabThreads) fox_page_tables_kernel(const TableParams p, const bool place) {
   __shared__ int64_t s_warp[kTabWarps];
+  __shared__ int32_t s_starts[kTabThreads + 1], s_granted[kTabThreads], s_lengths[kTabThreads], s_taken[kTabThreads];
+  __shared__ int s_served;
+  if (threadIdx.x == 0) s_served = s_starts[0] = 0;
   wait_for_kernel_in_front();
   const int free_before = max(0, min(*p.num_free, p.n_free_max));
   const int64_t page_less_1 = (1 << p.page_log2) - 1;
-  int64_t tokens = 0, taken = 0, served = 0;
+  const bool staged = p.R <= kTabThreads;   // all requests in shared memory
+  int64_t tokens = 0, taken = 0;
   for (int base = 0; base < p.R; base += kTabThreads) {
     const int r = base + threadIdx.x;
     const bool in = r < p.R;
@@ -102,29 +113,44 @@ __global__ void __launch_bounds__(kTabThreads) fox_page_tables_kernel(const Tabl
     const int64_t upto = taken + block_scan(need, sum, s_warp);
     taken += sum;
     const bool ok = fits && (need == 0 || upto <= free_before);
-    int64_t given;
-    block_scan(ok ? need : 0, given, s_warp);
-    served += given;
+    if (ok && need) atomicMax(&s_served, static_cast<int>(upto));   // (those that get pages are the first ones that need any)
     if (in) {
-      p.starts[r + 1] = clamp31(end);
+      const int start = clamp31(end), given = ok ? static_cast<int>(fresh) : 0, length = static_cast<int>(old) + given,
+                front = clamp31(upto - need);
+      p.starts[r + 1] = start;
       if (r == 0) p.starts[0] = 0;
-      p.granted[r] = ok ? static_cast<int>(fresh) : 0;
-      p.work[r] = clamp31(upto - need);
-      p.lengths_out[r] = static_cast<int>(old + (ok ? fresh : 0));
+      p.granted[r] = given;
+      p.lengths_out[r] = length;
+      if (staged) {
+        s_starts[r + 1] = start;
+        s_granted[r] = given;
+        s_lengths[r] = length;
+        s_taken[r] = front;
+      }
+      p.work[r] = front;
     }
   }
+  __syncthreads();
   if (threadIdx.x == 0) {
     p.work[p.R] = free_before;
-    *p.num_free_out = static_cast<int>(free_before - served);
+    *p.num_free_out = free_before - s_served;
   }
   if (!place) return;
-  __syncthreads();
-  for (int t = threadIdx.x; t < p.max_tokens; t += kTabThreads) place_token(p, t);
+  const Placing a = staged ? Placing{s_starts, s_granted, s_lengths, s_taken, free_before}
+                           : Placing{p.starts, p.granted, p.lengths_out, p.work, free_before};
+  for (int t = threadIdx.x; t < p.max_tokens; t += kTabThreads) place_token(p, a, t);
 }
+constexpr int kPlaceStaged = 4096;   // requests whose starts a block keeps
 __global__ void __launch_bounds__(256) fox_page_slots_kernel(const TableParams p) {
+  __shared__ int32_t s_starts[kPlaceStaged + 1];
   wait_for_kernel_in_front();
+  const bool staged = p.R <= kPlaceStaged;
+  if (staged)
+    for (int i = threadIdx.x; i <= p.R; i += 256) s_starts[i] = p.starts[i];
+  __syncthreads();
+  const Placing a{staged ? s_starts : p.starts, p.granted, p.lengths_out, p.work, p.work[p.R]};
   const int64_t t = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (t < p.max_tokens) place_token(p, static_cast<int>(t));
+  if (t < p.max_tokens) place_token(p, a, static_cast<int>(t));
 }
 
 // One CTA.  The pages behind keep[r] tokens go back on the stack, in the order of requests and of their tables' entries.

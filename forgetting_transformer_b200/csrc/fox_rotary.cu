@@ -22,8 +22,8 @@
 //            channels a thread and the other ones by shuffle, the kernels were bound by shared memory and shuffles: 66 us
 //            for what takes 48.)
 //   kNext    neighbouring channels paired: 8 neighbouring channels
-//   kAny     halves that are no multiple of 4: 8 neighbouring channels, the others of the pairs read from the row again, one by
-//            one (L1 has it)
+//   kAny     halves that are no multiple of 4: 8 neighbouring channels, the others of the pairs by way of shared memory, where the
+//            angles stand once for each channel (read from L1 again one by one: 214 us for what takes 83 so)
 #include "fox_common.cuh"
 #include "fox_host.h"
 
@@ -35,7 +35,8 @@ constexpr int kRotThreads = 256;
 constexpr int kRotTile = 32;      // tokens whose angles are in shared memory at a time
 constexpr int kRotAhead = 4;      // tokens whose rows a thread has asked for
 constexpr int64_t kRotTokens = (int64_t{1} << 31) - 65536;   // counted with 32 bits, a tile's more among them
-constexpr int kRotFwdPerSm = 4, kRotBwdPerSm = 2;   // CTAs, by registers
+__host__ __device__ constexpr int rot_fwd_per_sm(int mode) { return mode == kAny ? 3 : 4; }   // CTAs, by registers
+constexpr int kRotBwdPerSm = 2;
 
 struct RotaryTensor {
   const uint16_t *x, *dy;
@@ -53,6 +54,7 @@ struct RotaryParams {
   float* dw_partial;              // (shares, heads, D)
   float scale, sign, eps;         // sign: of the sine
   Divisor by_half;
+  int fold;                       // dw: both weights are one for all heads
   int pos_64, half, D, T, tokens, H, heads, heads_here, per_cta, tile;   // per_cta: tokens
 };
 
@@ -126,9 +128,11 @@ __device__ __forceinline__ float2 rot_mul(float2 a, float2 b) { return __fmul2_r
 __device__ __forceinline__ float2 rot_fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float2 rot_both(float a) { return make_float2(a, a); }
 
-// cosines and sines of tokens t0 .. t0 + n of sequence b, (tile, D / 2) each; s_pos: (tile).  A barrier is inside and one behind.
+// cosines and sines of tokens t0 .. t0 + n of sequence b, (tile, D / 2) each, kAny: (tile, D), a sine with the sign of its channel;
+// s_pos: (tile).  A barrier is inside and one behind.
+template <int kMode>
 __device__ __forceinline__ void rot_angles(const RotaryParams& p, int b, int t0, int n, double* s_pos, float* s_cos, float* s_sin) {
-  const int pairs = p.D >> 1;
+  const int ld = kMode == kAny ? p.D : p.D >> 1;
   for (int u = threadIdx.x; u < n; u += blockDim.x) {
     const int t = t0 + u;
     int64_t pos = p.first + t * p.step;
@@ -150,17 +154,22 @@ __device__ __forceinline__ void rot_angles(const RotaryParams& p, int b, int t0,
       // less whole turns, 2 pi in two parts
       const float r = static_cast<float>(fma(turns, -2.4492935982947064e-16, fma(turns, -6.283185307179586, a)));
       // (the fast functions: off by 2^-21 at most from minus pi to pi, far below half a step of 16 bits)
-      s_cos[u * pairs + f] = __cosf(r) * p.scale;
-      s_sin[u * pairs + f] = __sinf(r) * (p.scale * p.sign);
+      const float cs = __cosf(r) * p.scale, sn = __sinf(r) * (p.scale * p.sign);
+      s_cos[u * ld + f] = cs;
+      s_sin[u * ld + f] = kMode == kAny ? -sn : sn;
+      if constexpr (kMode == kAny) {
+        s_cos[u * ld + p.half + f] = cs;
+        s_sin[u * ld + p.half + f] = sn;
+      }
     }
   }
   __syncthreads();
 }
 
-// The rotation of a thread's 8 channels n; other(d): the value of channel d (kAny).
-template <int kMode, class Other>
+// The rotation of a thread's 8 channels n; pair: the other channels of their pairs (kAny).
+template <int kMode>
 __device__ __forceinline__ void rot_turn(const RotaryParams& p, const RotaryRuns& at, const float* c, const float* s, const float2* n,
-                                         Other&& other, float2* out) {
+                                         const float* pair, float2* out) {
   if constexpr (kMode == kHalves) {
     if (at.turned) {
       const float4 cv = *reinterpret_cast<const float4*>(c + at.a), sv = *reinterpret_cast<const float4*>(s + at.a);
@@ -190,27 +199,43 @@ __device__ __forceinline__ void rot_turn(const RotaryParams& p, const RotaryRuns
       }
     }
   } else {
-    auto one = [&](int d, float v) {
-      if (d >= 2 * p.half) return v;
-      const bool low = d < p.half;
-      const int i = low ? d : d - p.half;
-      const float m = other(low ? d + p.half : i);
-      return v * c[i] + m * (low ? -s[i] : s[i]);
-    };
+    float cv[8], sv[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) out[j] = make_float2(one(at.a + 2 * j, n[j].x), one(at.a + 2 * j + 1, n[j].y));
+    for (int i = 0; i < 2; ++i) {
+      *reinterpret_cast<float4*>(cv + 4 * i) = *reinterpret_cast<const float4*>(c + at.a + 4 * i);
+      *reinterpret_cast<float4*>(sv + 4 * i) = *reinterpret_cast<const float4*>(s + at.a + 4 * i);
+    }
+    auto one = [&](int j, float v) { return at.a + j < 2 * p.half ? v * cv[j] + pair[j] * sv[j] : v; };
+#pragma unroll
+    for (int j = 0; j < 4; ++j) out[j] = make_float2(one(2 * j, n[j].x), one(2 * j + 1, n[j].y));
   }
+}
+
+// kAny: a warp's packed values go to `slot` (512 bytes), and each thread takes the other channels of its pairs from there.
+__device__ __forceinline__ int rot_other(const RotaryParams& p, int d) {
+  return d < p.half ? d + p.half : d < 2 * p.half ? d - p.half : d;
+}
+template <bool kBf16>
+__device__ __forceinline__ void rot_exchange(const RotaryParams& p, uint16_t* slot, int lanes, int ch, const uint4& v, float* pair) {
+  const int lane = threadIdx.x & 31;
+  *reinterpret_cast<uint4*>(slot + lane * 8) = v;
+  __syncwarp();
+  const uint16_t* row = slot + (lane & ~(lanes - 1)) * 8;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) pair[j] = unpack2<kBf16>(row[rot_other(p, ch + j)]).x;
 }
 
 // grid: (ranges of per_cta tokens, blocks of heads_here heads); blockDim.x = heads_here * D / 8 up to a whole warp.  One wave of
 // CTAs with equal ranges, each in tiles of one sequence's tokens: of tiles as CTAs (16 tokens, 2.3 waves of them) the
 // norm of 2 x 8192 tokens x 32 heads of 128 took 74 us.
 template <bool kBf16, int kMode, bool kNorm, int kD>
-__global__ void __launch_bounds__(kRotThreads, kRotFwdPerSm) fox_rotary_fwd_kernel(const RotaryParams p) {
+__global__ void __launch_bounds__(kRotThreads, rot_fwd_per_sm(kMode)) fox_rotary_fwd_kernel(const RotaryParams p) {
+  constexpr int kAhead = kMode == kAny ? 2 : kRotAhead;
   extern __shared__ __align__(16) float rot_smem[];
-  const int D = kD ? kD : p.D, lanes = D >> 3, pairs = D >> 1;
+  const int D = kD ? kD : p.D, lanes = D >> 3, pairs = kMode == kAny ? D : D >> 1;
   double* s_pos = reinterpret_cast<double*>(rot_smem);
   float *s_cos = rot_smem + 2 * kRotTile, *s_sin = s_cos + p.tile * pairs;
+  uint16_t* s_rows = reinterpret_cast<uint16_t*>(s_sin + p.tile * pairs) + (threadIdx.x >> 5) * (kAhead * 256);   // kAny: of this warp
   const int sub = threadIdx.x % lanes, slot = threadIdx.x / lanes, head = blockIdx.y * p.heads_here + slot;
   const bool active = slot < p.heads_here && head < p.heads;
   const bool is_k = active && head >= p.H;
@@ -220,6 +245,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotFwdPerSm) fox_rotary_fwd_kern
   wait_for_kernel_in_front();
   const int begin = static_cast<int>(blockIdx.x) * p.per_cta, end = min(begin + p.per_cta, p.tokens);
   float2 w[4];
+  float wp[8];   // kAny: of the other channels
   const int64_t x_st = x.x_st, y_st = x.y_st;
   const float inv_d = 1.f / static_cast<float>(D);
   for (int at = begin, n; at < end; at += n) {
@@ -228,34 +254,44 @@ __global__ void __launch_bounds__(kRotThreads, kRotFwdPerSm) fox_rotary_fwd_kern
     const uint16_t* row = x.x + b * x.x_sb + h * x.x_sh + t0 * x.x_st;
     uint16_t* to = x.y + b * x.y_sb + h * x.y_sh + t0 * x.y_st;
     int to_ask = active ? n : 0;
-    uint4 ahead[kRotAhead];
+    uint4 ahead[kAhead];
     auto ask = [&] {
 #pragma unroll
-      for (int u = 0; u < kRotAhead; ++u) ahead[u] = u < to_ask ? rot_load<kMode>(row + u * x_st, ch) : make_uint4(0, 0, 0, 0);
-      row += kRotAhead * x_st;
-      to_ask -= kRotAhead;
+      for (int u = 0; u < kAhead; ++u) ahead[u] = u < to_ask ? rot_load<kMode>(row + u * x_st, ch) : make_uint4(0, 0, 0, 0);
+      row += kAhead * x_st;
+      to_ask -= kAhead;
     };
     ask();
     if constexpr (kNorm) {
       if (at == begin) {
         rot_weights(x.w, x.w_dtype, h * x.w_sh + ch.a, w);
         rot_weights(x.w, x.w_dtype, h * x.w_sh + ch.b, w + 2);
+        if constexpr (kMode == kAny)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) wp[j] = rot_weight(x.w, x.w_dtype, h * x.w_sh + rot_other(p, ch.a + j));
       }
     }
     if (at != begin) __syncthreads();   // (the last tile's angles have been used)
-    rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
+    rot_angles<kMode>(p, b, t0, n, s_pos, s_cos, s_sin);
     const float *c = s_cos, *s = s_sin;
-    for (int left = n; left > 0; left -= kRotAhead) {
-      uint4 raw[kRotAhead];
+    for (int left = n; left > 0; left -= kAhead) {
+      uint4 raw[kAhead];
 #pragma unroll
-      for (int u = 0; u < kRotAhead; ++u) raw[u] = ahead[u];
+      for (int u = 0; u < kAhead; ++u) raw[u] = ahead[u];
       ask();
 #pragma unroll
-      for (int u = 0; u < kRotAhead; ++u) {
+      for (int u = 0; u < kAhead; ++u) {
         if (u >= left) break;   // (the same for all threads)
         float2 v[4], out[4];
-        float r = 1.f;
+        float r = 1.f, pair[8];
         rot_unpack<kBf16>(raw[u], v);
+        if constexpr (kMode == kAny) {
+          rot_exchange<kBf16>(p, s_rows + u * 256, lanes, ch.a, raw[u], pair);
+          if constexpr (kNorm) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) pair[j] *= wp[j];
+          }
+        }
         if constexpr (kNorm) {
           float2 sq = rot_mul(v[0], v[0]);
 #pragma unroll
@@ -267,20 +303,17 @@ __global__ void __launch_bounds__(kRotThreads, kRotFwdPerSm) fox_rotary_fwd_kern
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = rot_mul(v[j], w[j]);
         }
-        auto other = [&](int d) {   // (row is two batches on)
-          const float m = active ? rot_weight(row + (u - 2 * kRotAhead) * x_st, kBf16 ? FOX_DTYPE_BF16 : FOX_DTYPE_FP16, d) : 0.f;
-          return kNorm ? m * rot_weight(x.w, x.w_dtype, h * x.w_sh + d) : m;
-        };
-        rot_turn<kMode>(p, ch, c + u * pairs, s + u * pairs, v, other, out);
+        rot_turn<kMode>(p, ch, c + u * pairs, s + u * pairs, v, pair, out);
         if constexpr (kNorm) {   // (1 / rms last: it is the same for both channels of a pair)
 #pragma unroll
           for (int j = 0; j < 4; ++j) out[j] = rot_mul(out[j], rot_both(r));
         }
         if (active) rot_store<kMode>(to + u * y_st, ch, rot_pack<kBf16>(out));
       }
-      to += kRotAhead * y_st;
-      c += kRotAhead * pairs;
-      s += kRotAhead * pairs;
+      if constexpr (kMode == kAny) __syncwarp();   // (the rows have been read before the next ones are written)
+      to += kAhead * y_st;
+      c += kAhead * pairs;
+      s += kAhead * pairs;
     }
   }
 }
@@ -291,9 +324,10 @@ template <bool kBf16, int kMode, int kD>
 __global__ void __launch_bounds__(kRotThreads, kRotBwdPerSm) fox_rotary_bwd_kernel(const RotaryParams p) {
   constexpr int kAhead = 2;
   extern __shared__ __align__(16) float rot_smem[];
-  const int D = kD ? kD : p.D, lanes = D >> 3, pairs = D >> 1;
+  const int D = kD ? kD : p.D, lanes = D >> 3, pairs = kMode == kAny ? D : D >> 1;
   double* s_pos = reinterpret_cast<double*>(rot_smem);
   float *s_cos = rot_smem + 2 * kRotTile, *s_sin = s_cos + p.tile * pairs;
+  uint16_t* s_rows = reinterpret_cast<uint16_t*>(s_sin + p.tile * pairs) + (threadIdx.x >> 5) * (kAhead * 256);   // kAny: of this warp
   const int sub = threadIdx.x % lanes, slot = threadIdx.x / lanes, head = blockIdx.y * p.heads_here + slot;
   const bool active = slot < p.heads_here && head < p.heads;
   const bool is_k = active && head >= p.H;
@@ -329,7 +363,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotBwdPerSm) fox_rotary_bwd_kern
       };
       ask();
       if (at != begin) __syncthreads();   // (the last tile's angles have been used)
-      rot_angles(p, b, t0, n, s_pos, s_cos, s_sin);
+      rot_angles<kMode>(p, b, t0, n, s_pos, s_cos, s_sin);
       const float *c = s_cos, *s = s_sin;
       for (int left = n; left > 0; left -= kAhead) {
         uint4 raw_x[kAhead], raw_g[kAhead];
@@ -345,10 +379,9 @@ __global__ void __launch_bounds__(kRotThreads, kRotBwdPerSm) fox_rotary_bwd_kern
           float2 v[4], g[4], dn[4], gw[4], out[4];
           rot_unpack<kBf16>(raw_x[u], v);
           rot_unpack<kBf16>(raw_g[u], g);
-          auto other = [&](int d) {   // (row_g is two batches on)
-            return active ? rot_weight(row_g + (u - 2 * kAhead) * dy_st, kBf16 ? FOX_DTYPE_BF16 : FOX_DTYPE_FP16, d) : 0.f;
-          };
-          rot_turn<kMode>(p, ch, c + u * pairs, s + u * pairs, g, other, dn);
+          float pair[8];
+          if constexpr (kMode == kAny) rot_exchange<kBf16>(p, s_rows + u * 256, lanes, ch.a, raw_g[u], pair);
+          rot_turn<kMode>(p, ch, c + u * pairs, s + u * pairs, g, pair, dn);
           float2 sq = rot_both(0.f), dot2 = rot_both(0.f);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -372,20 +405,36 @@ __global__ void __launch_bounds__(kRotThreads, kRotBwdPerSm) fox_rotary_bwd_kern
           }
           if (active) rot_store<kMode>(to + u * y_st, ch, rot_pack<kBf16>(out));
         }
+        if constexpr (kMode == kAny) __syncwarp();   // (the rows have been read before the next ones are written)
         to += kAhead * y_st;
         c += kAhead * pairs;
         s += kAhead * pairs;
       }
     }
   }
-  if (active) {
-    float* to = p.dw_partial + (static_cast<int64_t>(blockIdx.x) * p.heads + head) * p.D;
+  if (p.fold) {   // weights that all heads share: the heads of this CTA added up first, (ranges, blocks, 2, D)
+    __syncthreads();
+    float* s_dw = rot_smem;
+    if (active) {
+      *reinterpret_cast<float4*>(s_dw + slot * D + ch.a) = make_float4(dw[0].x, dw[0].y, dw[1].x, dw[1].y);
+      *reinterpret_cast<float4*>(s_dw + slot * D + ch.b) = make_float4(dw[2].x, dw[2].y, dw[3].x, dw[3].y);
+    }
+    __syncthreads();
+    const int first = blockIdx.y * p.heads_here, slots = min(p.heads_here, p.heads - first), of_q = min(max(p.H - first, 0), slots);
+    for (int i = threadIdx.x; i < 2 * D; i += blockDim.x) {
+      const int which = i >= D, d = i - which * D;
+      float sum = 0.f;
+      for (int j = which ? of_q : 0; j < (which ? slots : of_q); ++j) sum += s_dw[j * D + d];
+      p.dw_partial[((static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * 2 + which) * D + d] = sum;
+    }
+  } else if (active) {
+    float* to = p.dw_partial + (static_cast<int64_t>(blockIdx.x) * p.heads + head) * D;
     *reinterpret_cast<float4*>(to + ch.a) = make_float4(dw[0].x, dw[0].y, dw[1].x, dw[1].y);
     *reinterpret_cast<float4*>(to + ch.b) = make_float4(dw[2].x, dw[2].y, dw[3].x, dw[3].y);
   }
 }
 
-// dw of both tensors: 16 columns a CTA, its rows (shares, and heads where the weight is one for all) over 16 groups of threads
+// dw of both tensors: 16 columns a CTA, its rows (shares, and heads where one weight is one for all) over 32 groups of threads
 struct RotaryDwParams {
   const float* partial;
   void* dw[2];
@@ -394,28 +443,23 @@ struct RotaryDwParams {
   int heads[2];
   int n_partials, D;
 };
-__global__ void __launch_bounds__(256) fox_rotary_dw_kernel(const RotaryDwParams p) {
-  __shared__ float s_sum[16][17];
+__global__ void __launch_bounds__(512) fox_rotary_dw_kernel(const RotaryDwParams p) {
+  __shared__ float s_sum[32][17];
   wait_for_kernel_in_front();
   const int col = threadIdx.x & 15, grp = threadIdx.x >> 4;
   const int cols0 = p.shared[0] ? p.D : p.heads[0] * p.D;
   const int c_all = blockIdx.x * 16 + col, which = blockIdx.x * 16 >= cols0, c = c_all - (which ? cols0 : 0);
-  const int heads_all = p.heads[0] + p.heads[1];
-  const int64_t base = (which ? static_cast<int64_t>(p.heads[0]) * p.D : 0) + c, ld = static_cast<int64_t>(heads_all) * p.D;
+  const int64_t ld = static_cast<int64_t>(p.heads[0] + p.heads[1]) * p.D;
+  const float* from = p.partial + (which ? static_cast<int64_t>(p.heads[0]) * p.D : 0) + c;
   float sum = 0.f;
-  if (p.shared[which]) {
-    for (int h = 0; h < p.heads[which]; ++h)
-#pragma unroll 4
-      for (int r = grp; r < p.n_partials; r += 16) sum += p.partial[r * ld + base + h * p.D];
-  } else {
-#pragma unroll 4
-    for (int r = grp; r < p.n_partials; r += 16) sum += p.partial[r * ld + base];
-  }
+  for (int h = 0; h < (p.shared[which] ? p.heads[which] : 1); ++h)
+#pragma unroll 8
+    for (int r = grp; r < p.n_partials; r += 32) sum += from[r * ld + h * p.D];
   s_sum[grp][col] = sum;
   __syncthreads();
   if (grp == 0) {
 #pragma unroll
-    for (int g = 1; g < 16; ++g) sum += s_sum[g][col];
+    for (int g = 1; g < 32; ++g) sum += s_sum[g][col];
     if (p.w_dtype[which] == FOX_DTYPE_FP32) static_cast<float*>(p.dw[which])[c] = sum;
     else
       static_cast<uint16_t*>(p.dw[which])[c] =
@@ -424,6 +468,7 @@ __global__ void __launch_bounds__(256) fox_rotary_dw_kernel(const RotaryDwParams
 }
 
 // ------------------------------------------------------------------- launches
+static RotaryMode rotary_mode(int64_t half, int interleaved) { return interleaved ? kNext : half % 4 ? kAny : kHalves; }
 struct RotaryGrid {
   int blocks, heads_here, threads, ranges, per_cta, tile;
 };
@@ -453,10 +498,13 @@ static int rotary_launch_at(RotaryKind kind, dim3 grid, unsigned threads, size_t
 }
 static int rotary_launch(RotaryKind kind, int dtype, int64_t half, int interleaved, const RotaryGrid& g, cudaStream_t st, RotaryParams p) {
   p.heads_here = g.heads_here;
-  p.tile = g.tile;
+  p.tile = rotary_mode(half, interleaved) == kAny && g.tile > 16 ? 16 : g.tile;   // (two angles to a channel)
   p.per_cta = g.per_cta;
   const dim3 grid(g.ranges, g.blocks);
-  const size_t smem = kRotTile * sizeof(double) + static_cast<size_t>(p.tile) * p.D * sizeof(float);
+  const bool any = rotary_mode(half, interleaved) == kAny;
+  size_t smem = kRotTile * sizeof(double) + static_cast<size_t>(p.tile) * p.D * sizeof(float) * (any ? 2 : 1);
+  if (any) smem += g.threads / 32 * 2 * 512;
+  if (p.fold && smem < static_cast<size_t>(p.heads_here) * p.D * sizeof(float)) smem = static_cast<size_t>(p.heads_here) * p.D * sizeof(float);
   const bool bf = dtype == FOX_DTYPE_BF16;
   if (interleaved) return bf ? rotary_launch_at<true, kNext>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kNext>(kind, grid, g.threads, smem, st, p);
   if (half % 4) return bf ? rotary_launch_at<true, kAny>(kind, grid, g.threads, smem, st, p) : rotary_launch_at<false, kAny>(kind, grid, g.threads, smem, st, p);
@@ -523,7 +571,7 @@ extern "C" int fox_rotary(int device, void* stream, int dtype, int64_t B, int64_
   p.sign = inverse ? -1.f : 1.f;
   rotary_in(p.t[0], rotary_view(x, folded));
   rotary_out(p.t[0], rotary_view(y, folded));
-  return rotary_launch(kTurn, dtype, half, interleaved, rotary_grid(H, D, B * T, kRotFwdPerSm), (cudaStream_t)stream, p);
+  return rotary_launch(kTurn, dtype, half, interleaved, rotary_grid(H, D, B * T, rot_fwd_per_sm(rotary_mode(half, interleaved))), (cudaStream_t)stream, p);
 }
 
 extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
@@ -543,7 +591,7 @@ extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64
   rotary_out(p.t[0], rotary_view(q_out, folded)); rotary_out(p.t[1], rotary_view(k_out, folded));
   p.t[0].w = wq; p.t[0].w_dtype = wq_dtype; p.t[0].w_sh = wq_sh;
   p.t[1].w = wk; p.t[1].w_dtype = wk_dtype; p.t[1].w_sh = wk_sh;
-  return rotary_launch(kNormTurn, dtype, half, interleaved, rotary_grid(H + Hk, D, B * T, kRotFwdPerSm), (cudaStream_t)stream, p);
+  return rotary_launch(kNormTurn, dtype, half, interleaved, rotary_grid(H + Hk, D, B * T, rot_fwd_per_sm(rotary_mode(half, interleaved))), (cudaStream_t)stream, p);
 }
 
 extern "C" int64_t fox_qk_norm_rotary_partials(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D) {
@@ -581,10 +629,13 @@ extern "C" int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64
   p.t[0].w = wq; p.t[0].w_dtype = wq_dtype; p.t[0].w_sh = wq_sh;
   p.t[1].w = wk; p.t[1].w_dtype = wk_dtype; p.t[1].w_sh = wk_sh;
   p.dw_partial = dw_partial;
+  p.fold = !wq_sh && !wk_sh;
   const RotaryGrid g = rotary_grid(H + Hk, D, B * T, kRotBwdPerSm);
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = rotary_launch(kNormBack, dtype, half, interleaved, g, st, p)) return rc;
-  const RotaryDwParams d{dw_partial, {dwq, dwk}, {wq_dtype, wk_dtype}, {wq_sh == 0, wk_sh == 0}, {(int)H, (int)Hk}, g.ranges, (int)D};
+  const RotaryDwParams d = p.fold ? RotaryDwParams{dw_partial, {dwq, dwk}, {wq_dtype, wk_dtype}, {0, 0}, {1, 1}, g.ranges * g.blocks, (int)D}
+                                  : RotaryDwParams{dw_partial, {dwq, dwk}, {wq_dtype, wk_dtype}, {wq_sh == 0, wk_sh == 0}, {(int)H, (int)Hk},
+                                                   g.ranges, (int)D};
   const int64_t cols = (wq_sh ? H * D : D) + (wk_sh ? Hk * D : D);
-  return launch_behind(fox_rotary_dw_kernel, dim3((unsigned)(cols / 16)), 256, 0, st, d);
+  return launch_behind(fox_rotary_dw_kernel, dim3((unsigned)(cols / 16)), 512, 0, st, d);
 }

@@ -21,6 +21,14 @@ void same_device(const char* what, const Tensor& first, std::initializer_list<co
   for (const Tensor* t : others)
     if (t->defined() && t->device() != first.device()) raise_assert(std::string(what) + ": all tensors must be on one device");
 }
+// n elements of a contiguous vector from `at` on, as a tensor of its own over the same memory.  (at::narrow, with the autograd and
+// dispatch layers around it, costs a microsecond each; integers have no gradients.)
+Tensor run_of(const Tensor& all, int64_t at, int64_t n) {
+  Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), all.dtype());
+  t.unsafeGetTensorImpl()->set_storage_offset(all.storage_offset() + at);
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 void written(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
@@ -475,11 +483,11 @@ FOX_PY(py_page_tables) {
     const int64_t own = inplace ? 0 : R + 1;
     const Tensor all = at::empty({own + 2 * R + 1 + 3 * T + R + 1}, lengths.options());
     int32_t* base = all.mutable_data_ptr<int32_t>();
-    out[0] = inplace ? lengths : all.narrow(0, 0, R);
-    out[1] = inplace ? num_free : all.narrow(0, R, 1);
-    out[2] = all.narrow(0, own, R + 1);
-    out[3] = all.narrow(0, own + R + 1, R);
-    for (int i = 0; i < 3; ++i) out[4 + i] = all.narrow(0, own + 2 * R + 1 + i * T, T);
+    out[0] = inplace ? lengths : run_of(all, 0, R);
+    out[1] = inplace ? num_free : run_of(all, R, 1);
+    out[2] = run_of(all, own, R + 1);
+    out[3] = run_of(all, own + R + 1, R);
+    for (int i = 0; i < 3; ++i) out[4 + i] = run_of(all, own + 2 * R + 1 + i * T, T);
     int32_t *tokens = base + own + 2 * R + 1, *len_out = inplace ? lengths.mutable_data_ptr<int32_t>() : base,
             *free_out = inplace ? num_free.mutable_data_ptr<int32_t>() : base + R;
     launch("fox_page_tables", st, [&] {
