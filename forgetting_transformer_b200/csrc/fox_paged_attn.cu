@@ -58,7 +58,6 @@ struct PagedParams {
   uint16_t* o;
   float* L;                            // (R, H) or nullptr
   float* part;                         // (CTAs, 2, rows, D + 4), then (CTAs, warps, 2, rows, D + 4)
-  int* before;                         // (R + 1): places of a unit in front of every request
   int R, H, group, rows, tiles_of_group, units, n_pages, page_log2;   // rows: of a unit; units: of a request
   int32_t* status;
   Divisor by_units, by_tiles_of_group;
@@ -201,14 +200,6 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   s_before[tid + 1] = incl;
   if (tid == 0) s_before[0] = 0;
   __syncthreads();
-  if (blockIdx.x == 0) {
-    int at = incl - mine;
-    for (int r = r_first; r < r_end; ++r) {
-      p.before[r] = at;
-      at += pag_places(pag_length(p, r));
-    }
-    if (tid == 0) p.before[p.R] = s_before[kThreads];
-  }
   // ---- requests without a key
   for (int r = blockIdx.x; r < p.R; r += gridDim.x) {
     if (share == 1 ? s_length[r] : pag_length(p, r)) continue;
@@ -620,23 +611,52 @@ __global__ void __launch_bounds__(kJoinThreads) fox_paged_join_kernel(const Page
   constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kAhead = 8;
   __shared__ float s_w[kPagGrid], s_l[kPagGrid], s_g[kPagGrid], s_sum, s_top;
   __shared__ float4 s_o[kJoinThreads];
+  __shared__ int s_sum_before[kJoinThreads / 32], s_sum_all[kJoinThreads / 32];
   const int tid = threadIdx.x, sub = tid % kLanes, g0 = tid / kLanes;
-  wait_for_kernel_in_front();
-  const int per = pag_per_cta(p.before[p.R] * p.units);
-  for (int64_t item = blockIdx.x; item < static_cast<int64_t>(p.R) * p.H; item += gridDim.x) {
+  // Lengths may be read before the first kernel has ended: it has waited for what wrote them.
+  bool waited = false;
+  const int64_t items = static_cast<int64_t>(p.R) * p.H;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
     const int r = static_cast<int>(item < (int64_t{1} << 31) ? static_cast<uint32_t>(item) / static_cast<uint32_t>(p.H) : item / p.H);
     const int h = static_cast<int>(item - static_cast<int64_t>(r) * p.H);
-    const int before = p.before[r];
     const int places = pag_places(pag_length(p, r));
     if (places <= pag_whole(D)) continue;
+    int before = 0, all = 0;
+    for (int i = tid; i < p.R; i += kJoinThreads) {
+      const int n = pag_places(pag_length(p, i));
+      all += n;
+      if (i < r) before += n;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+      all += __shfl_xor_sync(0xffffffffu, all, o);
+    }
+    if ((tid & 31) == 0) {
+      s_sum_before[tid >> 5] = before;
+      s_sum_all[tid >> 5] = all;
+    }
+    __syncthreads();
+    before = all = 0;
+#pragma unroll
+    for (int i = 0; i < kJoinThreads / 32; ++i) {
+      before += s_sum_before[i];
+      all += s_sum_all[i];
+    }
+    const int per = pag_per_cta(all * p.units);
     const int kh = h / p.group, row = h - kh * p.group, unit = kh * p.tiles_of_group + row / kPagRows;
     const int u0 = before * p.units + unit * places;
     const int w0 = pag_div(u0 + kPagStart, per), n = pag_div(u0 + places - 1, per) - w0 + 1;
+    __syncthreads();   // (the sums have been read)
     if (n == 1) continue;
     const int64_t ld = static_cast<int64_t>(p.rows) * (D + 4);
     const float* base = p.part + (static_cast<int64_t>(w0) * 2 * p.rows + row % kPagRows) * (D + 4);
     const int second = w0 * per < u0;   // the first part's place: its CTA's range has begun in another unit
     auto at = [&](int s) { return base + (2 * s + (s == 0 ? second : 0)) * ld; };
+    if (!waited) {
+      wait_for_kernel_in_front();
+      waited = true;
+    }
     float4 ahead[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -710,6 +730,7 @@ __global__ void __launch_bounds__(kJoinThreads) fox_paged_join_kernel(const Page
     if (tid == 0 && p.L) p.L[item] = s_sum != 0.f ? s_top * kPagLn2 + __logf(s_sum) : -INFINITY;
     __syncthreads();   // (what is shared: the next pair's)
   }
+  if (!waited) wait_for_kernel_in_front();   // (this grid's end has to mean the first kernel's)
 }
 
 // (64 columns, rows of a page, halves, heads, pages); a head dim below 64: the columns behind it are filled with zeros
@@ -757,7 +778,7 @@ static int64_t paged_rows(int64_t H, int64_t Hk) { return H / Hk < kPagRows ? H 
 
 extern "C" int64_t fox_paged_attn_workspace_floats(int64_t R, int64_t H, int64_t Hk, int64_t D) {
   if (R <= 0 || H <= 0 || Hk <= 0 || D <= 0) return 1;
-  return R + 1 + 4 + kPagGrid * 2 * (1 + pag_warps(D)) * paged_rows(H, Hk) * (D + 4);
+  return kPagGrid * 2 * (1 + pag_warps(D)) * paged_rows(H, Hk) * (D + 4);
 }
 
 extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t n_pages,
@@ -788,8 +809,7 @@ extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, in
   p.gates = gate_pages; p.g_sp = gp_sp; p.g_sh = gp_sh;
   p.table = block_table; p.table_ld = table_ld; p.lengths = lengths;
   p.o = (uint16_t*)o; p.o_sr = o_sr; p.o_sh = o_sh; p.L = L;
-  p.before = reinterpret_cast<int*>(workspace);
-  p.part = workspace + (R + 1 + 3) / 4 * 4;
+  p.part = workspace;
   p.R = (int)R; p.H = (int)H; p.group = (int)(H / Hk); p.rows = (int)paged_rows(H, Hk);
   p.tiles_of_group = (p.group + kPagRows - 1) / kPagRows;
   p.units = (int)Hk * p.tiles_of_group;
