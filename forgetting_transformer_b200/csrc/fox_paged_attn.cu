@@ -38,10 +38,13 @@
 namespace fox {
 
 constexpr int kPagGrid = kSms;
-__host__ __device__ constexpr int pag_warps(int64_t D) { return D == 128 ? 8 : 16; }
+// Warps of a CTA, each with two tiles asked for: some 110 and 140 KB in flight on an SM.  More is slower, since SMs then get more
+// uneven shares of the bandwidth (24 x 65536 keys of 64: 12 warps x 2 tiles 70.5 us, 16 x 3 76; 32 x 2048 x 16 heads of 128: 8 x 2
+// 91, 8 x 3 98, 10 x 2 94), fewer warps too (8 x 4 88).
+__host__ __device__ constexpr int pag_warps(int64_t D) { return D == 128 ? 8 : 12; }
 constexpr int kPagTile = 16;
 constexpr int kPagRows = 8;          // query heads of a unit
-constexpr int kPagStart = 2;         // what the start of a unit costs, in tiles
+constexpr int kPagStart = 1;         // what the start of a unit costs, in tiles
 constexpr int kPagLeast = 3;         // places of a warp
 // Units of up to so many places are one CTA's: some 280 KB of keys and values, which one SM reads in the time that parts of several
 // CTAs take to be joined.
@@ -134,7 +137,7 @@ struct PagedTile {
   static constexpr int kStage = 2 * kHalves * kBox;           // keys, values
   static constexpr int kGates = kPagRows * kPagTile * 4;
   static constexpr int kCols = D / 8;                         // n of the second product
-  static constexpr int kStages = 3;
+  static constexpr int kStages = 2;
   static constexpr int kWarps = pag_warps(D), kThreads = kWarps * 32;
   static constexpr int kSmem = kWarps * kStages * (kStage + kGates) + 1024;   // (boxes begin at multiples of 1024 bytes)
 };
@@ -551,22 +554,23 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
         v[s][0] = in ? *at_v : 0.f;
       }
     }
+    constexpr int kUp = kWarps > 8 ? 16 : 8;   // lanes that the shuffles below go over
     float behind = st.z, y;   // gates of the parts from this one on
 #pragma unroll
-    for (int o = 1; o < kWarps; o <<= 1) {
+    for (int o = 1; o < kUp; o <<= 1) {
       y = __shfl_down_sync(0xffffffffu, behind, o);
-      if (lane + o < kWarps) behind += y;
+      if (lane + o < kUp) behind += y;
     }
     const float all = __shfl_sync(0xffffffffu, behind, 0);
     y = __shfl_down_sync(0xffffffffu, behind, 1);
-    const float mm = lane < n ? st.x + (lane + 1 < kWarps ? y : 0.f) : -INFINITY;
+    const float mm = lane < n ? st.x + (lane + 1 < kUp ? y : 0.f) : -INFINITY;
     float top = mm;
 #pragma unroll
-    for (int o = kWarps / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int o = kUp / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float w = mm == -INFINITY ? 0.f : fast_exp2(mm - top);   // (NaN stays)
     float sum = st.y * w;
 #pragma unroll
-    for (int o = kWarps / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    for (int o = kUp / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     float acc[kPer];
 #pragma unroll
     for (int c_i = 0; c_i < kPer; ++c_i) acc[c_i] = 0.f;
