@@ -3,7 +3,8 @@
 Mirrors the data flow of upstream's ``ForgettingAttentionLayer`` / ``ForgettingTransformerMLP`` /
 ``ForgettingTransformerBlock`` (modeling_forgetting_transformer.py:98-430, 467-516, 519-622) in the "Pro"
 configuration: output gate + output norm, per-head QK-norm, data-dependent K and V token shift, full forget
-gate, no rotary embedding; training path and, with an ``FgateCache``, the prefill / generation path.
+gate, rotary positions where they are asked for (upstream's ``use_rope``); training path and, with an ``FgateCache``, the
+prefill / generation path.
 
 A plain block without a cache, and a generated token with one, run natively (csrc/host_block.cpp): the projections of a
 sequence are one cuBLASLt product with stacked weights, those of a token kernels of this library.  Everything else runs the
@@ -26,6 +27,7 @@ import torch.nn.functional as F
 from . import _lib
 from .cache import FgateCache, _LayerStore
 from .norm_gate import FusedGroupNormGated, GroupNorm, RMSNorm
+from .rotary import RotaryEmbedding
 from .ops import (acp_threshold_from_qk_norm, forgetting_attention, forgetting_attention_from_gate_logits,
                   seq_start_from_attention_mask)
 from .glu import swiglu_linear_packed
@@ -84,9 +86,11 @@ class FoxProAttentionLayer(nn.Module):
 
     def __init__(self, hidden_size: int, num_heads: int, norm_eps: float = 1e-6, qk_norm: bool = True,
                  use_k_shift: bool = True, use_v_shift: bool = True, fgate_bias: float = 0.0,
-                 log_pruning_tolerance: Optional[float] = None, initializer_range: float = 0.02):
+                 log_pruning_tolerance: Optional[float] = None, initializer_range: float = 0.02,
+                 rotary: Optional[RotaryEmbedding] = None):
         super().__init__()
         assert hidden_size % num_heads == 0
+        self.rotary = rotary
         self.hidden_size, self.num_heads, self.head_dim = hidden_size, num_heads, hidden_size // num_heads
         self.q_proj = nn.Linear(hidden_size, hidden_size, bias=False)
         self.k_proj = (ShiftLinear(hidden_size, hidden_size, num_heads) if use_k_shift
@@ -138,7 +142,17 @@ class FoxProAttentionLayer(nn.Module):
         q = self.q_proj(hidden_states)
         k = self.k_proj(hidden_states, step_mask, k_state) if self.use_k_shift else self.k_proj(hidden_states)
         v = self.v_proj(hidden_states, step_mask, v_state) if self.use_v_shift else self.v_proj(hidden_states)
-        if self.qk_norm:
+        rotary = getattr(self, "rotary", None)   # (a layer pickled before there were any has none)
+        if rotary is not None:              # positions count on from the history (upstream lines 318-331)
+            past = 0 if past_key_values is None else past_key_values.get_seq_length(layer_idx)
+            q, k = q.view(B, T, H, D), k.view(B, T, H, D)
+            if self.qk_norm and self.q_norm.eps == self.k_norm.eps:
+                q, k = rotary.norm(q, k, self.q_norm.weight, self.k_norm.weight, past, eps=self.q_norm.eps)
+            else:
+                if self.qk_norm:
+                    q, k = [n(x.flatten(2)).view(B, T, H, D) for n, x in ((self.q_norm, q), (self.k_norm, k))]
+                q, k = rotary(q, k, past)
+        elif self.qk_norm:
             q = self.q_norm(q).to(q.dtype)
             k = self.k_norm(k).to(k.dtype)
         fgate_logit = self.fgate_proj(hidden_states).transpose(1, 2)               # (B, H, T) view
@@ -186,11 +200,12 @@ class FoxProBlock(nn.Module):
     """attn_norm -> attention -> (residual add + mlp_norm, prenorm) -> MLP -> residual add (upstream lines 552-622)."""
 
     def __init__(self, hidden_size: int = 1536, num_heads: int = 24, intermediate_size: int = 4096,
-                 norm_eps: float = 1e-6, fgate_bias: float = 0.0, log_pruning_tolerance: Optional[float] = None):
+                 norm_eps: float = 1e-6, fgate_bias: float = 0.0, log_pruning_tolerance: Optional[float] = None,
+                 rotary: Optional[RotaryEmbedding] = None):
         super().__init__()
         self.attn_norm = RMSNorm(hidden_size, eps=norm_eps)
         self.attn = FoxProAttentionLayer(hidden_size, num_heads, norm_eps=norm_eps, fgate_bias=fgate_bias,
-                                         log_pruning_tolerance=log_pruning_tolerance)
+                                         log_pruning_tolerance=log_pruning_tolerance, rotary=rotary)
         self.mlp_norm = RMSNorm(hidden_size, eps=norm_eps)
         self.mlp = FoxMLP(hidden_size, intermediate_size)
 
@@ -204,8 +219,11 @@ class FoxProBlock(nn.Module):
         """hidden_states (B, T, hidden) in fp16/bf16 (the residual stream is kept in that dtype here).
 
         Without a cache the whole block runs as one native forward and backward where its parts are the plain modules
-        built here (no hooks, replaced submodules or autocast) in one 16-bit dtype; else module by module."""
-        if past_key_values is None:
+        built here (no hooks, replaced submodules or autocast) in one 16-bit dtype; else, and with rotary positions, module by
+        module."""
+        if getattr(self.attn, "rotary", None) is not None:
+            pass
+        elif past_key_values is None:
             out = (_host or _load_host()).block(self, hidden_states, attention_mask, self._threshold)
             if out is not None:
                 return out

@@ -259,3 +259,55 @@ def test_rotary_module(scaling):
         n = norm64(x.double(), 0.5, 1e-5)
         ref = turn64(n, a, False, s)
         assert ((got.double() - ref).abs() <= 2 ** -8 * ref.abs() + 2 ** -19 * reach(n, 32, False, s)).all()
+
+
+def composed(layer, x, cache=None, layer_idx=0):
+    """The attention layer from its modules and the public operators, as its documentation has it."""
+    B, T, C = x.shape
+    H, D = layer.num_heads, layer.head_dim
+    past = cache.get_seq_length(layer_idx) if cache is not None else 0
+    k_state, v_state = (cache.key_shift_cache[layer_idx], cache.value_shift_cache[layer_idx]) if cache is not None else (None, None)
+    q, k, v = layer.q_proj(x), layer.k_proj(x, None, k_state), layer.v_proj(x, None, v_state)
+    q, k = layer.rotary.norm(q.view(B, T, H, D), k.view(B, T, H, D), layer.q_norm.weight, layer.k_norm.weight, past, eps=layer.q_norm.eps)
+    q, k, v = [t.reshape(B, T, H, D).transpose(1, 2) for t in (q, k, v)]
+    logit = layer.fgate_proj(x).transpose(1, 2)
+    if cache is None:
+        o = fox.forgetting_attention_from_gate_logits(q, k, v, logit, head_first=True, sm_scale=D ** -0.5)
+    else:
+        k, v, g = cache.update(k, v, torch.nn.functional.logsigmoid(logit.float()), layer_idx)
+        o = fox.forgetting_attention(q, k, v, g, head_first=True, sm_scale=D ** -0.5)
+    return layer.o_proj(layer.output_norm(o.transpose(1, 2).reshape(B, T, C), layer.ogate_proj(x)))
+
+
+def test_layer_with_rotary_positions():
+    """The layer with rotary positions is its modules with ``RotaryEmbedding.norm`` in the norms' place: the same calls, so the
+    same bits, forward, backward and with a cache; a block with such a layer does not take the native path, which has none."""
+    torch.manual_seed(0)
+    block = fox.FoxProBlock(256, 4, 512, rotary=fox.RotaryEmbedding(64, 10000.0)).cuda().bfloat16()
+    plain = fox.FoxProBlock(256, 4, 512).cuda().bfloat16()
+    plain.load_state_dict(block.state_dict())
+    x = data(1, 2, 37, 256, dtype=torch.bfloat16)
+    layer = block.attn
+    grads = []
+    for f in (lambda y: layer(y), lambda y: composed(layer, y)):
+        layer.zero_grad()
+        xin = x.clone().requires_grad_()
+        out = f(xin)
+        out.backward(data(2, *out.shape, dtype=torch.bfloat16))
+        grads.append([out.detach(), xin.grad] + [p.grad.clone() for p in layer.parameters()])
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+    with torch.no_grad():
+        out = block(x)
+        h, res = block.mlp_norm(layer(block.attn_norm(x)), x, True)
+        assert torch.equal(out, res + block.mlp(h))
+        assert not torch.equal(out, plain(x))
+        caches = []
+        for f in (layer, composed):
+            cache = fox.FgateCache(64)
+            s = layer.init_shift_state(2)
+            cache.update_shift_cache(s["key_shift"], s["value_shift"], 0)
+            call = (lambda y: layer(y, None, cache, 0)) if f is layer else (lambda y: composed(layer, y, cache))
+            caches.append([call(x[:, :30])] + [call(x[:, t:t + 1]) for t in range(30, 37)])
+        for a, b in zip(*caches):
+            assert torch.equal(a, b)
