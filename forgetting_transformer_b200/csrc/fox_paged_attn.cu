@@ -805,6 +805,10 @@ extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, in
       off(v_pages->ptr, v_pages->sb, v_pages->sh, v_pages->st, 8) || off(gate_pages, gp_sp, gp_sh, 0, 4) ||
       off(o, o_sr, o_sh, 0, 8) || reinterpret_cast<uintptr_t>(workspace) % 16)
     return FOX_ERR_ALIGNMENT;
+  // places are counted with 30 bits: so many requests at a time, going by what their table rows could hold
+  const int64_t tiles_of_group = (H / Hk + kPagRows - 1) / kPagRows, most = width * page < 2147483647LL - 64 ? width * page : 2147483647LL - 64;
+  const int64_t at_once = (int64_t{1} << 30) / (Hk * tiles_of_group * ((most + kPagTile - 1) / kPagTile + kPagStart));
+  if (at_once < 1) return FOX_ERR_TOO_LARGE;
   if (cudaSetDevice(device) != cudaSuccess) return FOX_ERR_DEVICE;
   PagedParams p{};
   p.q = (const uint16_t*)q;
@@ -815,17 +819,14 @@ extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, in
   p.o = (uint16_t*)o; p.o_sr = o_sr; p.o_sh = o_sh; p.L = L;
   p.part = workspace;
   p.R = (int)R; p.H = (int)H; p.group = (int)(H / Hk); p.rows = (int)paged_rows(H, Hk);
-  p.tiles_of_group = (p.group + kPagRows - 1) / kPagRows;
+  p.tiles_of_group = (int)tiles_of_group;
   p.units = (int)Hk * p.tiles_of_group;
   p.by_units = divisor(p.units);
   p.by_tiles_of_group = divisor(p.tiles_of_group);
   p.n_pages = (int)n_pages;
   for (p.page_log2 = 4; (int64_t{1} << p.page_log2) < page;) ++p.page_log2;
-  p.most = width * page < 2147483647LL - 64 ? width * page : 2147483647LL - 64;
+  p.most = most;
   p.qk_scale = sm_scale * kPagLog2e;
-  // places are counted with 30 bits: so many requests at a time, going by what their table rows could hold
-  const int64_t places = p.units * ((p.most + kPagTile - 1) / kPagTile + kPagStart), at_once = (int64_t{1} << 30) / places;
-  if (at_once < 1) return FOX_ERR_TOO_LARGE;
   cudaStream_t st = (cudaStream_t)stream;
   const bool bf = dtype == FOX_DTYPE_BF16;
   CUtensorMap mk, mv;

@@ -78,6 +78,8 @@ fox_tensor4 rows_t4(const Tensor& x, bool head_first) {
 }
 void check_rotation(Rotation& r, const Rows& s, const Tensor& x, const char* what) {
   check_that(r.inv_freq.dim() == 1 && r.inv_freq.scalar_type() == at::kFloat, "inv_freq must be a vector in torch.float32");
+  if (at::GradMode::is_enabled() && r.inv_freq.requires_grad())
+    raise_fox(std::string(what) + " has no gradient for inv_freq: detach it, or call it under torch.no_grad()");
   r.half = r.inv_freq.numel();
   check_that(r.half >= 1 && 2 * r.half <= s.D, "inv_freq must have between 1 and head dim / 2 elements");
   if (r.positions.defined()) {

@@ -507,7 +507,7 @@ int fox_paged_update(int device, void* stream, int64_t T, int64_t H, int64_t Hk,
 /* Forward attention of one query row per request, q (R, H, D), against its lengths[r] keys (0: out 0, L -inf); query head h reads
  * key head h / (H / Hk) and its own gates.  A table entry outside the pool leaves its keys out.  o (R, H, D); L (R, H) fp32 or
  * NULL; gate strides multiples of 4; workspace: fox_paged_attn_workspace_floats(...), 16-byte aligned;
- * status as for fox_attn_fwd. */
+ * status as for fox_attn_fwd.  A table row that could hold more than 2^30 tiles of 16 keys over all heads: FOX_ERR_TOO_LARGE. */
 int64_t fox_paged_attn_workspace_floats(int64_t R, int64_t H, int64_t Hk, int64_t D);
 int fox_paged_attn(int device, void* stream, int dtype, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t n_pages, int64_t page,
                    int64_t width, const void* q, int64_t q_sr, int64_t q_sh, const fox_tensor4* k_pages,

@@ -351,6 +351,30 @@ def test_same_page_in_two_requests():
     check(queries(8, 2, 2, 64, torch.bfloat16), kp, vp, gp, table, n)
 
 
+def test_very_wide_tables():
+    """Tables whose rows could hold more tiles than are counted at a time: the requests go in several launches."""
+    lengths = [40, 0, 1000, 17, 3, 0, 5000, 64, 65, 1]
+    kp, vp, gp, table, n = pool_of(40, lengths, 16, 16, 64, 64, torch.bfloat16)
+    wide = torch.full((len(lengths), 2 ** 21), -7, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    q = queries(9, len(lengths), 16, 64, torch.bfloat16)
+    got = fox.paged_forgetting_attention(q, kp, vp, gp, wide, n, return_log_normalizer=True)
+    check(q, kp, vp, gp, table, n, None, got)
+
+
+def test_inference_mode():
+    cache = fox.PagedFgateCache(1, 8, 16, 2, 64, 2, 50)
+    with torch.inference_mode():
+        t = cache.extend(i32([3, 20]), 30)
+        k = torch.randn(30, 2, 64, generator=gen(1)).bfloat16().cuda()
+        cache.update(0, k, k, -torch.ones(30, 2, device="cuda"), t.slots)
+        out = cache.attend(0, k[:2])
+        cache.release(torch.tensor([True, False], device="cuda"))
+    check(k[1:2], *cache[0], cache.block_table[1:], cache.lengths[1:], None,
+          (out[1:], fox.paged_forgetting_attention(k[1:2], *cache[0], cache.block_table[1:], cache.lengths[1:], return_log_normalizer=True)[1]))
+    assert cache.lengths.tolist() == [0, 20] and cache.num_free.tolist() == [6]
+
+
 def test_streams_and_graphs():
     """Two captured calls on streams of their own, replayed side by side on new values, against plain calls; results of a call
     do not change from one to the next."""

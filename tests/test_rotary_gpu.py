@@ -213,6 +213,29 @@ def test_one_result_unused_and_frozen_inputs():
         torch.autograd.grad(out[1].float().sum(), [k])
 
 
+def test_inference_mode_and_the_traced_functions():
+    """Under inference_mode, and by the autograd functions that torch.jit.trace records: the same bits, gradients too."""
+    inv_freq, _ = fox.rotary_frequencies(64, device="cuda")
+    q, k = [data(i, 2, 13, 3, 64, dtype=torch.float16) for i in range(2)]
+    w = torch.rand(192, device="cuda") + 0.5
+    with torch.inference_mode():
+        a = [fox.rotary_embedding(q, inv_freq, 5), *fox.qk_norm_rotary(q, k, w, w, inv_freq, 5)]
+    pos = 5 + torch.arange(13, device="cuda")
+    f = lambda q, k, w: [fox.rotary_embedding(q, inv_freq, pos), *fox.qk_norm_rotary(q, k, w, w, inv_freq, pos)]
+    traced = torch.jit.trace(f, (q, k, w), check_trace=False)
+    for x, y in zip(a, traced(q, k, w)):
+        assert torch.equal(x, y)
+    leaves = [t.clone().requires_grad_() for t in (q, k, w)]
+    dy = [data(7 + i, 2, 13, 3, 64, dtype=torch.float16) for i in range(3)]
+    from forgetting_transformer_b200 import rotary
+    args = (inv_freq, pos, False, False, 1.0)
+    by_class = [rotary._Rotate.apply(leaves[0], *args), *rotary._NormRotate.apply(leaves[0], leaves[1], leaves[2], leaves[2], inv_freq, pos, 1e-5, False, False, 1.0)]
+    got = torch.autograd.grad(by_class, leaves, dy)
+    want = torch.autograd.grad(f(*leaves), leaves, dy)
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+
+
 def test_streams_and_graphs():
     """On a stream of the caller's, forward and backward captured in a graph and replayed on new values."""
     inv_freq, _ = fox.rotary_frequencies(64, device="cuda")

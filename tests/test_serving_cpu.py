@@ -53,6 +53,16 @@ def test_no_cpu_path():
         fox.paged_forgetting_attention(bf(3, 2, 64), *pool, i(3, 4), i(3))
 
 
+def test_frequencies_have_no_gradient():
+    f = F32.clone().requires_grad_()
+    with pytest.raises(_lib.FoxError, match="no gradient for inv_freq"):
+        fox.rotary_embedding(bf(1, 4, 2, 64), f)
+    with pytest.raises(_lib.FoxError, match="no gradient for inv_freq"):
+        fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 2, 64), torch.ones(64), torch.ones(64), f)
+    with torch.no_grad(), pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.rotary_embedding(bf(1, 4, 2, 64), f)
+
+
 def pages(P=5, Hk=2, H=2, page=16, D=64, dtype=torch.bfloat16):
     return (torch.zeros(P, Hk, page, D, dtype=dtype), torch.zeros(P, Hk, page, D, dtype=dtype), torch.zeros(P, H, page))
 
@@ -129,6 +139,7 @@ def test_c_interface_refuses_sizes():
                                                  gh=4, tab=a, ld=2, len=a, sc=1.0, o=a, orr=8, oh=8, L=None, ws=a, status=a), **c}.values())
     assert att(D=8) == -2 and att(H=3) == -1 and att(page=17) == -1 and att(ld=1) == -1 and att(P=2 ** 28) == -8 and att(gp=2) == -3
     assert att(R=0) == -1 and att(q=8) == -3 and att(ws=None) == -1 and att(status=None) == -1
+    assert att(H=64, Hk=64, page=65536, w=2 ** 15, ld=2 ** 15) == -8     # more than 2^30 tiles in one request
     assert lib.fox_paged_attn_workspace_floats(0, 1, 1, 64) == 1 and lib.fox_qk_norm_rotary_partials(0, 0, 0, 0, 0) == 1
 
 
