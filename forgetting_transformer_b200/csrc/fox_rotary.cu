@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kRotThreads, rot_fwd_per_sm(kMode)) fox_rotary
 // shares in a fixed order.
 template <bool kBf16, int kMode, int kD>
 __global__ void __launch_bounds__(kRotThreads, kRotBwdPerSm) fox_rotary_bwd_kernel(const RotaryParams p) {
-  constexpr int kAhead = 2;
+  constexpr int kAhead = kMode == kAny ? 2 : kRotAhead;
   extern __shared__ __align__(16) float rot_smem[];
   const int D = kD ? kD : p.D, lanes = D >> 3, pairs = kMode == kAny ? D : D >> 1;
   double* s_pos = reinterpret_cast<double*>(rot_smem);
