@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kRotThreads, rot_fwd_per_sm(kMode)) fox_rotary
   const int h = active ? (is_k ? head - p.H : head) : 0;
   const RotaryRuns ch = rot_runs<kMode>(p, sub);
   wait_for_kernel_in_front();
-  const int begin = static_cast<int>(blockIdx.x) * p.per_cta, end = min(begin + p.per_cta, p.tokens);
+  const int begin = static_cast<int>(blockIdx.x) * p.per_cta, end = begin + min(p.per_cta, p.tokens - begin);
   float2 w[4];
   float wp[8];   // kAny: of the other channels
   const int64_t x_st = x.x_st, y_st = x.y_st;
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kRotThreads, kRotBwdPerSm) fox_rotary_bwd_kern
   for (int j = 0; j < 4; ++j) dw[j] = rot_both(0.f);
   const int64_t x_st = x.x_st, dy_st = x.dy_st, y_st = x.y_st;
   const float inv_d = 1.f / static_cast<float>(D);
-  const int begin = static_cast<int>(blockIdx.x) * p.per_cta, end = min(begin + p.per_cta, p.tokens);
+  const int begin = static_cast<int>(blockIdx.x) * p.per_cta, end = begin + min(p.per_cta, p.tokens - begin);
   for (int at = begin, n; at < end; at += n) {
     const int b = at / p.T, t0 = at - b * p.T;
     n = min(min(p.tile, end - at), p.T - t0);
