@@ -40,8 +40,9 @@ namespace fox {
 constexpr int kPagGrid = kSms;
 // Warps of a CTA, each with two tiles asked for: some 110 and 140 KB in flight on an SM.  More is slower, since SMs then get more
 // uneven shares of the bandwidth (24 x 65536 keys of 64: 12 warps x 2 tiles 70.5 us, 16 x 3 76; 32 x 2048 x 16 heads of 128: 8 x 2
-// 91, 8 x 3 98, 10 x 2 94), fewer warps too (8 x 4 88).
-__host__ __device__ constexpr int pag_warps(int64_t D) { return D == 128 ? 8 : 12; }
+// 91, 8 x 3 98, 10 x 2 94), fewer warps too (8 x 4 88).  Head dims 16 and 32 are bound by what a tile takes a warp, not by its
+// bytes: 16 warps (16 requests of 1000 to 9000 keys x 16 heads of 32: 12 warps 45 us, 16 38).
+__host__ __device__ constexpr int pag_warps(int64_t D) { return D == 128 ? 8 : D == 64 ? 12 : 16; }
 constexpr int kPagTile = 16;
 constexpr int kPagRows = 8;          // query heads of a unit
 constexpr int kPagStart = 1;         // what the start of a unit costs, in tiles
