@@ -143,7 +143,7 @@ class FoxProAttentionLayer(nn.Module):
         k = self.k_proj(hidden_states, step_mask, k_state) if self.use_k_shift else self.k_proj(hidden_states)
         v = self.v_proj(hidden_states, step_mask, v_state) if self.use_v_shift else self.v_proj(hidden_states)
         rotary = getattr(self, "rotary", None)   # (a layer pickled before there were any has none)
-        if rotary is not None:              # positions count on from the history (upstream lines 318-331)
+        if rotary is not None:              # positions count on from the history
             past = 0 if past_key_values is None else past_key_values.get_seq_length(layer_idx)
             q, k = q.view(B, T, H, D), k.view(B, T, H, D)
             if self.qk_norm and self.q_norm.eps == self.k_norm.eps:

@@ -8,7 +8,7 @@
 //   backward: dn = the rotation by -a of dy;  dw_h += dn xhat (xhat = x rstd);  dx = rstd (dn w - xhat mean_d(dn w xhat))
 //
 // Upstream norms q and k in one kernel (layernorm.py:183-245 as modeling_forgetting_transformer.py:264-265, 314-316 builds
-// it) and rotates them in another (rotary.py:22-153, from a table of cosines and sines in the tensors' type); here the
+// it) and rotates them in another (rotary.py:22-153, from tables of cosines and sines); here the
 // normed values are never rounded or written in between, and one launch takes both tensors.
 //
 // There is no table of all positions: a CTA forms the angles of its own tile of tokens, once for all of its heads.  The

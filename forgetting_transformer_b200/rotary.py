@@ -1,8 +1,7 @@
 """Rotary positions, alone and with the per-head RMSNorm of queries and keys in the same pass.
 
-Upstream's ``RotaryEmbedding`` (model/forgetting_transformer/rotary.py:156-553; the layer's ``use_rope``,
-modeling_forgetting_transformer.py:266-268, 318-331) rotates from a table of cosines and sines in the tensors' type that
-grows with the longest position; here the kernel forms the angles of the positions that it meets, product and reduction in
+Upstream's rotary embedding (model/forgetting_transformer/rotary.py, kernel 22-153; the layer's ``use_rope``) rotates by a
+kernel of its own, from tables of cosines and sines; here the kernel forms the angles of the positions that it meets, product and reduction in
 64 bits, so that there is no table and no longest position, and each value is rounded once.
 """
 from __future__ import annotations
@@ -128,7 +127,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
 
 class RotaryEmbedding(nn.Module):
     """Rotary positions of a layer: ``rotary_frequencies``' arguments, kept with the layout of the pairs.  ``forward`` rotates
-    q and k as upstream's module does (rotary.py:505-553); ``norm`` norms them first.  The frequencies stay in fp32 whatever
+    q and k; ``norm`` norms them first.  The frequencies stay in fp32 whatever
     type the module is moved to."""
 
     def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, **scaling):
