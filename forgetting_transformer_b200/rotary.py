@@ -48,7 +48,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Literal["non
         if dim == 2:
             raise ValueError("ntk scaling needs more than one frequency")
         base = base * factor ** (dim / (dim - 2))
-    freq = torch.pow(float(base), -torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    freq = torch.pow(float(base), -torch.arange(0, dim, 2, dtype=torch.float64, device="cpu") / dim)
     scale = 1.0
     if scaling == "linear":
         freq = freq / factor
@@ -59,7 +59,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, scaling: Literal["non
         kept = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0, 1)
         freq = freq * kept + freq / factor * (1 - kept)
         scale = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
-    return freq.to(torch.float32).to(device), scale
+    return freq.to(torch.float32).to(torch.get_default_device() if device is None else device), scale
 
 
 class _Rotate(torch.autograd.Function):
@@ -127,19 +127,26 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
 
 class RotaryEmbedding(nn.Module):
     """Rotary positions of a layer: ``rotary_frequencies``' arguments, kept with the layout of the pairs.  ``forward`` rotates
-    q and k; ``norm`` norms them first.  The frequencies stay in fp32 whatever
-    type the module is moved to."""
+    q and k; ``norm`` norms them first.  The frequencies stay in fp32 whatever type the module is moved to; they come from the
+    arguments, so that a module built on the meta device has them too, and what is pickled holds no device's copy."""
 
     def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, **scaling):
         super().__init__()
         self.dim, self.base, self.interleaved = dim, float(base), interleaved
-        self._freq, self.scale = rotary_frequencies(dim, base, **scaling)
+        with torch.inference_mode(False):
+            self._freq, self.scale = rotary_frequencies(dim, base, device="cpu", **scaling)
         self._on_device = {}
+
+    def __getstate__(self):
+        return {**self.__dict__, "_on_device": {}}
 
     def inv_freq(self, device) -> torch.Tensor:
         got = self._on_device.get(device)
         if got is None:
-            got = self._on_device[device] = self._freq.to(device)
+            with torch.inference_mode(False):   # (the copy serves training too)
+                got = self._freq.to(device)
+            if type(got) is torch.Tensor:       # (a tracer's stand-in is not kept)
+                self._on_device[device] = got
         return got
 
     def extra_repr(self) -> str:

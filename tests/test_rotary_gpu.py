@@ -334,3 +334,16 @@ def test_layer_with_rotary_positions():
             caches.append([call(x[:, :30])] + [call(x[:, t:t + 1]) for t in range(30, 37)])
         for a, b in zip(*caches):
             assert torch.equal(a, b)
+
+
+def test_module_trains_after_inference():
+    """Frequencies that came to the device under inference mode serve a backward pass afterwards."""
+    m = fox.RotaryEmbedding(32)
+    q, k = [data(i, 1, 9, 2, 64, dtype=torch.bfloat16) for i in range(2)]
+    with torch.inference_mode():
+        first = m(q, k, 3)
+    leaf = q.clone().requires_grad_()
+    out = m(leaf, k, 3)
+    assert torch.equal(out[0], first[0]) and torch.equal(out[1], first[1])
+    out[0].backward(torch.ones_like(leaf))
+    assert leaf.grad.abs().max() > 0

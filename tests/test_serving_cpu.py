@@ -1,5 +1,7 @@
 """Refusals of the rotary and paged-cache operators, which come before anything runs on a GPU, and the frequencies."""
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -163,3 +165,21 @@ def test_frequencies():
                 dict(dim=64, factor=0.0), dict(dim=2, scaling="ntk", factor=2.0)):
         with pytest.raises(ValueError):
             fox.rotary_frequencies(**bad)
+
+
+def test_module_keeps_its_frequencies():
+    """Built on the meta device or under inference mode, copied and pickled: the frequencies are the arguments' own, on any device
+    asked for, and no copy of one device goes with the module to another."""
+    want, _ = fox.rotary_frequencies(64, 500000.0)
+    cpu = torch.device("cpu")
+    with torch.device("meta"):
+        meta = fox.RotaryEmbedding(64, 500000.0)
+        assert fox.rotary_frequencies(64)[0].is_meta
+    with torch.inference_mode():
+        made = fox.RotaryEmbedding(64, 500000.0)
+        assert not made.inv_freq(cpu).is_inference()
+    used = fox.RotaryEmbedding(64, 500000.0)
+    used.inv_freq(cpu)
+    for m in (meta, made, used, copy.deepcopy(used), pickle.loads(pickle.dumps(used))):
+        assert torch.equal(m.inv_freq(cpu), want)
+    assert used._on_device and not pickle.loads(pickle.dumps(used))._on_device
