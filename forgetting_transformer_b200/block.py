@@ -165,7 +165,10 @@ class FoxProAttentionLayer(nn.Module):
         thr = None
         if self.log_pruning_tolerance is not None:
             assert self.qk_norm, "the closed-form threshold needs QK-norm"
-            thr = acp_threshold_from_qk_norm(self.q_norm.weight, self.k_norm.weight, H, D, N,
+            w_q = self.q_norm.weight
+            if rotary is not None and rotary.scale != 1:   # (q and k are both longer by the scale)
+                w_q = w_q * rotary.scale ** 2
+            thr = acp_threshold_from_qk_norm(w_q, self.k_norm.weight, H, D, N,
                                              self.log_pruning_tolerance)
         seq_start = None
         if attention_mask is not None:

@@ -6,6 +6,7 @@ by 2^-21.19 at most from minus pi to pi, and a turned value adds two products (2
 pair (a, b).  A norm's 1 / rms is off by half of its sum's error (8 + log2(D / 8) roundings of terms of one sign) and two ulp:
 below 2^-20 of its value, so that a normed pair gets 2^-19."""
 import itertools
+import math
 
 import pytest
 import torch
@@ -347,3 +348,20 @@ def test_module_trains_after_inference():
     assert torch.equal(out[0], first[0]) and torch.equal(out[1], first[1])
     out[0].backward(torch.ones_like(leaf))
     assert leaf.grad.abs().max() > 0
+
+
+def test_layer_with_scale_prunes_within_its_tolerance(monkeypatch):
+    """The closed-form threshold counts the rotation's scale, by which both q and k are longer: -(2 bound + ln T) + tolerance with
+    bound = scale^2 max|w_q| max|w_k| sqrt(D) (here 1 x 1 x 8)."""
+    from forgetting_transformer_b200 import block as block_module
+    rot = fox.RotaryEmbedding(64, scaling="yarn", factor=16.0, original_length=2048)
+    layer = fox.FoxProAttentionLayer(128, 2, log_pruning_tolerance=-10.0, rotary=rot).cuda().bfloat16()
+    seen = []
+    inner = block_module.forgetting_attention_from_gate_logits
+    monkeypatch.setattr(block_module, "forgetting_attention_from_gate_logits",
+                        lambda *a, **k: seen.append(k["adaptive_threshold"]) or inner(*a, **k))
+    with torch.no_grad():
+        layer(data(1, 1, 128, 128, dtype=torch.bfloat16))
+    want = -(2 * rot.scale ** 2 * 8 + math.log(128)) - 10
+    # the weights are 1 in bf16; scale^2, bound, sum and result are rounded to bf16: 4 x 2^-8, of terms up to |want|
+    assert rot.scale > 1.2 and (seen[0].double() - want).abs().max() <= 4 * 2 ** -8 * abs(want)
