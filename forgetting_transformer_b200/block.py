@@ -82,6 +82,15 @@ class ShiftLinear(nn.Module):
         return result.to(out.dtype).reshape(B, T, -1)
 
 
+def _plain_norm(n: nn.Module, num_heads: int) -> bool:
+    """Whether ``n`` is the norm that the layer builds, so that a kernel may stand in for calling it."""
+    m = nn.modules.module
+    return (type(n) is GroupNorm and n.is_rms_norm and n.weight is not None and n.num_groups == num_heads
+            and not (n._forward_hooks or n._forward_pre_hooks or n._backward_hooks or n._backward_pre_hooks or "forward" in n.__dict__)
+            and not (m._global_forward_hooks or m._global_forward_pre_hooks or m._global_backward_hooks
+                     or m._global_backward_pre_hooks))
+
+
 class FoxProAttentionLayer(nn.Module):
 
     def __init__(self, hidden_size: int, num_heads: int, norm_eps: float = 1e-6, qk_norm: bool = True,
@@ -146,11 +155,12 @@ class FoxProAttentionLayer(nn.Module):
         if rotary is not None:              # positions count on from the history
             past = 0 if past_key_values is None else past_key_values.get_seq_length(layer_idx)
             q, k = q.view(B, T, H, D), k.view(B, T, H, D)
-            if self.qk_norm and self.q_norm.eps == self.k_norm.eps:
+            norms = (self.q_norm, self.k_norm) if self.qk_norm else ()
+            if norms and all(_plain_norm(n, H) for n in norms) and self.q_norm.eps == self.k_norm.eps:
                 q, k = rotary.norm(q, k, self.q_norm.weight, self.k_norm.weight, past, eps=self.q_norm.eps)
             else:
-                if self.qk_norm:
-                    q, k = [n(x.flatten(2)).view(B, T, H, D) for n, x in ((self.q_norm, q), (self.k_norm, k))]
+                if norms:
+                    q, k = [n(x.flatten(2)).to(x.dtype).view(B, T, H, D) for n, x in zip(norms, (q, k))]
                 q, k = rotary(q, k, past)
         elif self.qk_norm:
             q = self.q_norm(q).to(q.dtype)

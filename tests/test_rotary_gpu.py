@@ -365,3 +365,28 @@ def test_layer_with_scale_prunes_within_its_tolerance(monkeypatch):
     want = -(2 * rot.scale ** 2 * 8 + math.log(128)) - 10
     # the weights are 1 in bf16; scale^2, bound, sum and result are rounded to bf16: 4 x 2^-8, of terms up to |want|
     assert rot.scale > 1.2 and (seen[0].double() - want).abs().max() <= 4 * 2 ** -8 * abs(want)
+
+
+def test_layer_calls_norms_that_are_not_its_own():
+    """Replaced norms of q and k, and those with hooks, are called; the rotation follows them."""
+    layer = fox.FoxProAttentionLayer(128, 2, rotary=fox.RotaryEmbedding(64)).cuda().bfloat16()
+    x = data(1, 1, 20, 128, dtype=torch.bfloat16)
+    calls = []
+
+    class Half(torch.nn.Module):
+        def forward(self, x):
+            calls.append("half")
+            return x / 2
+    with torch.no_grad():
+        fused = layer(x)
+        handle = layer.q_norm.register_forward_hook(lambda *a: calls.append("hook"))
+        hooked = layer(x)
+        handle.remove()
+        assert calls == ["hook"] and torch.equal(layer(x), fused) and calls == ["hook"]
+        norms = [fox.GroupNorm(2, 128, is_rms_norm=True).cuda().bfloat16() for _ in range(2)]
+        layer.rotary.norm = lambda q, k, w_q, w_k, past, eps: layer.rotary(
+            *[n(x.flatten(2)).view(x.shape) for n, x in zip(norms, (q, k))], past)
+        assert torch.equal(hooked, composed(layer, x))
+        del layer.rotary.norm
+        layer.q_norm = layer.k_norm = Half()
+        assert not torch.equal(layer(x), fused) and calls == ["hook", "half", "half"]
