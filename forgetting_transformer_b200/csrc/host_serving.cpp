@@ -248,6 +248,7 @@ NormSaved norm_inputs(const Tensor& q, const Tensor& k, const Tensor& wq, const 
   check_that(q.dim() == k.dim() && ks.B == a.s.B && ks.T == a.s.T && ks.D == a.s.D && k.scalar_type() == q.scalar_type(),
              "q and k must agree in batch, tokens, head dim and type");
   a.Hk = ks.H;
+  check_that(a.s.H >= 1 && a.Hk >= 1, "q and k must have one head at least");
   check_weight(wq, a.s.H, a.s.D, "q_weight");
   check_weight(wk, a.Hk, a.s.D, "k_weight");
   check_rotation(r, a.s, q, "qk_norm_rotary");

@@ -183,3 +183,10 @@ def test_module_keeps_its_frequencies():
     for m in (meta, made, used, copy.deepcopy(used), pickle.loads(pickle.dumps(used))):
         assert torch.equal(m.inv_freq(cpu), want)
     assert used._on_device and not pickle.loads(pickle.dumps(used))._on_device
+
+
+def test_no_heads_are_refused():
+    with pytest.raises(AssertionError, match="one head"):
+        fox.qk_norm_rotary(bf(1, 4, 0, 64), bf(1, 4, 2, 64), torch.ones(64), torch.ones(64), F32)
+    with pytest.raises(AssertionError, match="one head"):
+        fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 0, 64), torch.ones(64), torch.ones(64), F32)
