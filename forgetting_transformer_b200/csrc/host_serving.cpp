@@ -1,6 +1,7 @@
 // Rotary positions, the paged generation cache and its attention on the host: checks, allocations, launches, autograd nodes.
 #include "host_common.h"
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
 
 #include <array>
@@ -124,11 +125,12 @@ Tensor rotate(const Tensor& x_in, const Rotation& r, const Rows& s, bool inverse
   return y;
 }
 
+Tensor rotate_recorded(const Tensor& x, const Rotation& r, const Rows& s, bool inverse);
 struct Rotate : public torch::autograd::Node {
   SavedVariable inv_freq, positions;
   Rotation rest;   // (its tensors are left empty)
   Rows shape;
-  bool released = false;
+  bool inverse = false, released = false;
   std::string name() const override { return "RotaryEmbeddingBackward"; }
   void release_variables() override {
     inv_freq.reset_data();
@@ -141,9 +143,26 @@ struct Rotate : public torch::autograd::Node {
     Rotation r = rest;
     r.inv_freq = inv_freq.unpack();
     r.positions = positions.unpack();
-    return {rotate(grads[0], r, shape, true)};
+    return {rotate_recorded(grads[0], r, shape, !inverse)};
   }
 };
+// with a node where x has a gradient (in a backward pass: where that is differentiated)
+Tensor rotate_recorded(const Tensor& x, const Rotation& r, const Rows& s, bool inverse) {
+  const Tensor y = rotate(x, r, s, inverse);
+  if (at::GradMode::is_enabled() && x.requires_grad()) {
+    std::shared_ptr<Rotate> node(new Rotate(), torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    torch::autograd::set_history(y, node);
+    node->inv_freq = SavedVariable(r.inv_freq, false);
+    node->positions = SavedVariable(r.positions, false);
+    node->rest = r;
+    node->rest.inv_freq.reset();
+    node->rest.positions.reset();
+    node->shape = s;
+    node->inverse = inverse;
+  }
+  return y;
+}
 
 // ---------------------------------------------------------------- with the norm of q and k
 struct NormSaved {
@@ -237,6 +256,14 @@ struct NormRotate : public torch::autograd::Node {
     std::array<Tensor, 4> g = norm_backward(a, grads[0], grads[1]);
     for (size_t i = 0; i < 4; ++i)
       if (task_should_compute_output(i)) out[i] = g[i];
+    if (at::GradMode::is_enabled()) {   // (a second derivative is an error, not zero)
+      std::shared_ptr<torch::autograd::Error> second(
+          new torch::autograd::Error("qk_norm_rotary has no second derivative",
+                                     torch::autograd::collect_next_edges(a.q, a.k, a.wq, a.wk, grads[0], grads[1])),
+          torch::autograd::deleteNode);
+      for (Tensor& o : out)
+        if (o.defined()) torch::autograd::set_history(o, second);
+    }
     return out;
   }
 };
@@ -349,18 +376,7 @@ FOX_PY(py_rotary) {
     const Rows s = rows_of(x, r.head_first, "x");
     check_rotation(r, s, x, "rotary_embedding");
     status_poll(x.device().index());
-    y = rotate(x, r, s, false);
-    if (at::GradMode::is_enabled() && x.requires_grad()) {
-      std::shared_ptr<Rotate> node(new Rotate(), torch::autograd::deleteNode);
-      node->set_next_edges(torch::autograd::collect_next_edges(x));
-      torch::autograd::set_history(y, node);
-      node->inv_freq = SavedVariable(r.inv_freq, false);
-      node->positions = SavedVariable(r.positions, false);
-      r.inv_freq.reset();
-      r.positions.reset();
-      node->rest = std::move(r);
-      node->shape = s;
-    }
+    y = rotate_recorded(x, r, s, false);
   }
   return THPVariable_Wrap(y);
   END_HANDLE_TH_ERRORS

@@ -11,6 +11,7 @@ from typing import Literal, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -73,6 +74,7 @@ class _Rotate(torch.autograd.Function):
         return _lib.host().rotary_apply(x, inv_freq, positions, head_first, interleaved, scale, False)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         inv_freq, positions = ctx.saved_tensors
         at = positions if ctx.first is None else ctx.first
@@ -89,6 +91,7 @@ class _NormRotate(torch.autograd.Function):
         return _lib.host().qk_norm_rotary_forward(q, k, q_weight, k_weight, inv_freq, positions, *ctx.rest)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         *tensors, positions = ctx.saved_tensors
         at = positions if ctx.first is None else ctx.first
@@ -106,7 +109,7 @@ def rotary_embedding(x: torch.Tensor, inv_freq: torch.Tensor, positions: Positio
     - positions: (T,) or (B, T) int32 / int64 on the device, an int (the first token's), or None: 0, 1, 2, ...;
     - pairs: channels i and i + half, with ``interleaved`` channels 2 i and 2 i + 1.
 
-    Differentiable w.r.t. x."""
+    Differentiable w.r.t. x, any number of times."""
     pos = 0 if positions is None else positions
     out = (_host or _load_host()).rotary(x, inv_freq, pos, head_first, interleaved, scale)
     return _Rotate.apply(x, inv_freq, pos, head_first, interleaved, scale) if out is None else out
@@ -118,7 +121,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     """``rotary_embedding`` of the per-head RMSNorms of q and k (``GroupNorm``) in one kernel, without rounding between the two.
 
     q (B, T, H, D) and k (B, T, Hk, D), or (T, H, D), as for ``rotary_embedding``; q_weight (H * D,) or (D,) for all heads
-    alike, k_weight likewise, fp16 / bf16 / fp32.  Returns (q, k); differentiable w.r.t. q, k and both weights."""
+    alike, k_weight likewise, fp16 / bf16 / fp32.  Returns (q, k); differentiable, once, w.r.t. q, k and both weights."""
     pos = 0 if positions is None else positions
     out = (_host or _load_host()).qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, pos, eps, head_first, interleaved, scale)
     return (_NormRotate.apply(q, k, q_weight, k_weight, inv_freq, pos, eps, head_first, interleaved, scale)

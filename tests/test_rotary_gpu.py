@@ -390,3 +390,26 @@ def test_layer_calls_norms_that_are_not_its_own():
         del layer.rotary.norm
         layer.q_norm = layer.k_norm = Half()
         assert not torch.equal(layer(x), fused) and calls == ["hook", "half", "half"]
+
+
+def test_second_derivatives():
+    """The rotation's gradient is the rotation back, and that one's the rotation: |y|^2 / 2 has the gradient x (scale 1) and the second
+    derivative v along v, each value rounded twice.  The norms' second derivative is refused, not zero."""
+    inv_freq, _ = fox.rotary_frequencies(64, device="cuda")
+    x = data(1, 1, 9, 2, 64, dtype=torch.bfloat16).requires_grad_()
+    v = data(2, 1, 9, 2, 64, dtype=torch.bfloat16)
+    y = fox.rotary_embedding(x, inv_freq, 7)
+    (g,) = torch.autograd.grad((y * y).sum() / 2, [x], create_graph=True)
+    (h,) = torch.autograd.grad(g, [x], v)
+    for got, ref in ((g, x), (h, v)):
+        # the first rounding's half steps, turned, are 2^-8 of the turned pair's |a| + |b| at most, which is 2^0.5 of the pair's own
+        slack = (2 ** 0.5 * 2 ** -8 + 2 ** -19) * reach(ref.double(), 32, False)
+        assert ((got.double() - ref.double()).abs() <= 2 ** -8 * (ref.double().abs() + slack) + slack + 2 ** -7 * slack).all()
+    q, k = [data(i, 1, 9, 2, 64, dtype=torch.bfloat16).requires_grad_() for i in range(2)]
+    w = torch.ones(64, device="cuda")
+    out = fox.qk_norm_rotary(q, k, w, w, inv_freq)
+    g = torch.autograd.grad(out[0].float().pow(2).sum(), [q], create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+        torch.autograd.grad(g[0].float().sum(), [q])
+    out = fox.qk_norm_rotary(q, k, w, w, inv_freq)
+    assert not torch.autograd.grad(out[0].float().sum(), [q])[0].requires_grad
