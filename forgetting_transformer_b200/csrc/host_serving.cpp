@@ -318,7 +318,7 @@ PyObject* pair(const Tensor& a, const Tensor& b) {
 // ---------------------------------------------------------------- the paged cache
 bool page_size_ok(int64_t page) { return page >= 16 && page <= 65536 && !(page & (page - 1)); }
 void check_int32(const Tensor& t, int64_t dims, const char* what) {
-  if (t.dim() != dims || t.scalar_type() != at::kInt || t.stride(-1) != 1)
+  if (t.dim() != dims || t.scalar_type() != at::kInt || (t.size(-1) > 1 && t.stride(-1) != 1))
     raise_assert(std::string(what) + " must be in torch.int32, of " + std::to_string(dims) + " dimension" + (dims > 1 ? "s" : "") +
                  ", the last one contiguous");
 }

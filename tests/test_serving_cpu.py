@@ -190,3 +190,14 @@ def test_no_heads_are_refused():
         fox.qk_norm_rotary(bf(1, 4, 0, 64), bf(1, 4, 2, 64), torch.ones(64), torch.ones(64), F32)
     with pytest.raises(AssertionError, match="one head"):
         fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 0, 64), torch.ones(64), torch.ones(64), F32)
+
+
+def test_one_request_out_of_many_columns():
+    """Vectors of one element may carry any stride: they pass the checks that come before the device's."""
+    state = torch.zeros(1, 3, dtype=torch.int32)
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    assert state[:, 1].stride(0) == 3
+    with pytest.raises(_lib.FoxError, match="no CPU path"):
+        fox.page_tables(state[:, 0], state[:, 1], i(1, 3), i(5), state[:, 2], 16, 4)
+    with pytest.raises(AssertionError, match="contiguous"):
+        fox.page_tables(i(2, 3)[:, 0], i(2), i(2, 3), i(5), i(1), 16, 4)
