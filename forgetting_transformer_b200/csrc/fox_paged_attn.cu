@@ -10,8 +10,9 @@
 // cut into equal ranges for the CTAs of a grid that fills the GPU once, and each of these into equal ranges for its warps: the
 // longest request and the shortest cost what their tiles cost.  Every CTA sums up the lengths by itself before its first load and
 // finds its range there.  A unit of a few hundred keys is not cut between CTAs (its range is moved to the unit's end).  A unit
-// that lies in one warp's range is written at once; of one that is cut, each part's (o, m, l, sum of gates) goes to a workspace.
-// The CTA joins its warps' parts at its end, a second kernel the CTAs' parts.
+// that lies in one warp's range is written at once; of one that is cut, each part's (o, m, l, sum of gates) goes to shared memory.
+// The CTA joins its warps' parts at its end (from a workspace in global memory, 2 us later, with HBM busy), and a second kernel
+// the CTAs' parts, from a workspace.
 //
 // The bias of a key is the sum of the gates behind it.  A warp goes through its part of a unit from the right, so that this
 // is a running sum (exact where the bias is small, which is where it matters; a prefix sum over the whole request would lose
@@ -61,7 +62,7 @@ struct PagedParams {
   int64_t table_ld;
   uint16_t* o;
   float* L;                            // (R, H) or nullptr
-  float* part;                         // (CTAs, 2, rows, D + 4), then (CTAs, warps, 2, rows, D + 4)
+  float* part;                         // (CTAs, 2, rows, D + 4)
   int R, H, group, rows, tiles_of_group, units, n_pages, page_log2;   // rows: of a unit; units: of a request
   int32_t* status;
   Divisor by_units, by_tiles_of_group;
@@ -140,7 +141,8 @@ struct PagedTile {
   static constexpr int kCols = D / 8;                         // n of the second product
   static constexpr int kStages = 2;
   static constexpr int kWarps = pag_warps(D), kThreads = kWarps * 32;
-  static constexpr int kSmem = kWarps * kStages * (kStage + kGates) + 1024;   // (boxes begin at multiples of 1024 bytes)
+  static constexpr int kParts = kWarps * kStages * (kStage + kGates);   // where the warps' parts begin: (warps, 2, rows, D + 4)
+  static constexpr int kSmem = kParts + kWarps * 2 * kPagRows * (D + 4) * 4 + 1024;   // (boxes begin at multiples of 1024 bytes)
 };
 
 // What a stage's tile is: written by lane 0, read by the warp.
@@ -294,6 +296,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   char* const base = pag_smem + (smem0 - smem_u32(pag_smem));
   char* const ring = base + warp * kStages * Tile::kStage;
   float* const ring_g = reinterpret_cast<float*>(base + kWarps * kStages * Tile::kStage + warp * kStages * Tile::kGates);
+  float* const parts = reinterpret_cast<float*>(base + Tile::kParts);
   const int x = lane >> 2, c = lane & 3;
   // (rows of gates that no head fills: finite)
 #pragma unroll
@@ -483,7 +486,7 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
             *reinterpret_cast<uint32_t*>(to + j * 8 + 2 * c) = pack2<kBf16>((o[j][0] + o[j][2]) * inv, (o[j][1] + o[j][3]) * inv);
           if (p.L && c == 0) p.L[static_cast<int64_t>(item.r) * p.H + h] = ls != 0.f ? m_ref * kPagLn2 + __logf(ls) : -INFINITY;
         } else {
-          float* to = p.part + ((static_cast<int64_t>(2 * kPagGrid) + (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * 2 + (item.flags & kItemSecond ? 1 : 0)) * p.rows + x) * (D + 4);
+          float* to = parts + ((warp * 2 + (item.flags & kItemSecond ? 1 : 0)) * p.rows + x) * (D + 4);
 #pragma unroll
           for (int j = 0; j < Tile::kCols; ++j)
             *reinterpret_cast<float2*>(to + j * 8 + 2 * c) = make_float2(o[j][0] + o[j][2], o[j][1] + o[j][3]);
@@ -532,8 +535,8 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     const int kh_j = div_by(p.by_tiles_of_group, f.unit), in_group = (f.unit - kh_j * p.tiles_of_group) * kPagRows;
     const int h_j = kh_j * p.group + in_group + row_j;
     if (row_j >= p.group - in_group) continue;
-    const int64_t rows_ld = static_cast<int64_t>(p.rows) * (D + 4);
-    const float* from = p.part + (2 * kPagGrid + (static_cast<int64_t>(blockIdx.x) * kWarps + wa) * 2) * rows_ld + row_j * (D + 4);
+    const int rows_ld = p.rows * (D + 4);
+    const float* from = parts + wa * 2 * rows_ld + row_j * (D + 4);
     const bool second = c_begin + wa * per < f.at;   // the first part's place: its warp has begun in another unit
     auto part = [&](int s) { return from + 2 * s * rows_ld + (s == 0 && second ? rows_ld : 0); };
     // lane s: part s
@@ -783,7 +786,7 @@ static int64_t paged_rows(int64_t H, int64_t Hk) { return H / Hk < kPagRows ? H 
 
 extern "C" int64_t fox_paged_attn_workspace_floats(int64_t R, int64_t H, int64_t Hk, int64_t D) {
   if (R <= 0 || H <= 0 || Hk <= 0 || D <= 0) return 1;
-  return kPagGrid * 2 * (1 + pag_warps(D)) * paged_rows(H, Hk) * (D + 4);
+  return kPagGrid * 2 * paged_rows(H, Hk) * (D + 4);
 }
 
 extern "C" int fox_paged_attn(int device, void* stream, int dtype, int64_t R, int64_t H, int64_t Hk, int64_t D, int64_t n_pages,
