@@ -56,8 +56,8 @@ def page_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: to
       granted none and keeps its length; its tokens have slot -1, which ``paged_update`` leaves out.
     - ``inplace``: lengths and num_free are changed instead of returned anew.
     - page_size: a power of two from 16 to 65536."""
-    return PageTables(*(_host or _load_host()).page_tables(lengths, new_tokens, block_table, free_pages, num_free, page_size,
-                                                           max_tokens, inplace))
+    return PageTables._make((_host or _load_host()).page_tables(lengths, new_tokens, block_table, free_pages, num_free, page_size,
+                                                                max_tokens, inplace))
 
 
 def release_pages(lengths: torch.Tensor, keep: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
