@@ -472,15 +472,26 @@ static RotaryMode rotary_mode(int64_t half, int interleaved) { return interleave
 struct RotaryGrid {
   int blocks, heads_here, threads, ranges, per_cta, tile;
 };
-// Heads of a token over as few CTAs of up to 256 threads as hold them, evenly; tokens over as many ranges as make one wave.
-static RotaryGrid rotary_grid(int64_t heads, int64_t D, int64_t tokens, int per_sm) {
+enum RotaryKind { kTurn, kNormTurn, kNormBack };
+// Heads of a token over as few CTAs of up to 256 threads as hold them, evenly; tokens over as many ranges as make one wave.  CTAs of
+// fewer threads are more to an SM (36 heads of 64, 160 threads each: 61 -> 57 us, backward 104 -> 88), up to the threads that a kernel is
+// fastest with (24 heads of 64 rotated only, 192 threads: 4 CTAs 36.5 us, 5 37.2); where the weights' shares are added up
+// afterwards, while ranges keep 16 tokens (3000 tokens x 16 heads of 64: 8.9 us, of 6 tokens 11.2).
+static RotaryGrid rotary_grid(RotaryKind kind, bool any, int64_t heads, int64_t D, int64_t tokens) {
   const int64_t most = kRotThreads / (D / 8), blocks = (heads + most - 1) / most, here = (heads + blocks - 1) / blocks;
-  const int64_t fit = kSms * per_sm / blocks, want = fit < 1 ? 1 : fit, per = (tokens + want - 1) / want;
-  return {static_cast<int>(blocks), static_cast<int>(here), static_cast<int>((here * (D / 8) + 31) / 32 * 32),
+  const int64_t threads = (here * (D / 8) + 31) / 32 * 32;
+  const int64_t smem = kRotTile * (8 + D * 4) + threads / 32 * 1024 + 1024;   // of a CTA at most
+  const int64_t least = kind == kNormBack ? kRotBwdPerSm : rot_fwd_per_sm(any ? kAny : kHalves);   // CTAs to an SM
+  const int64_t by_threads = (kind == kNormBack ? 512 : kind == kTurn || any ? 768 : 1024) / threads, by_smem = 220 * 1024 / smem;
+  const int64_t more = by_threads < by_smem ? by_threads : by_smem;
+  auto ranges = [&](int64_t per_sm) { return kSms * per_sm / blocks < 1 ? 1 : kSms * per_sm / blocks; };
+  int64_t want = ranges(more > least ? more : least);
+  if (kind == kNormBack && tokens < 16 * want) want = ranges(least) > tokens / 16 ? ranges(least) : tokens / 16;
+  const int64_t per = (tokens + want - 1) / want;
+  return {static_cast<int>(blocks), static_cast<int>(here), static_cast<int>(threads),
           static_cast<int>((tokens + per - 1) / per), static_cast<int>(per), static_cast<int>(per < kRotTile ? per : kRotTile)};
 }
 
-enum RotaryKind { kTurn, kNormTurn, kNormBack };
 template <bool kBf16, int kMode, int kD>
 static int rotary_launch_of(RotaryKind kind, dim3 grid, unsigned threads, size_t smem, cudaStream_t st, const RotaryParams& p) {
   if (kind == kTurn) return launch_behind(fox_rotary_fwd_kernel<kBf16, kMode, false, kD>, grid, threads, smem, st, p);
@@ -571,7 +582,7 @@ extern "C" int fox_rotary(int device, void* stream, int dtype, int64_t B, int64_
   p.sign = inverse ? -1.f : 1.f;
   rotary_in(p.t[0], rotary_view(x, folded));
   rotary_out(p.t[0], rotary_view(y, folded));
-  return rotary_launch(kTurn, dtype, half, interleaved, rotary_grid(H, D, B * T, rot_fwd_per_sm(rotary_mode(half, interleaved))), (cudaStream_t)stream, p);
+  return rotary_launch(kTurn, dtype, half, interleaved, rotary_grid(kTurn, rotary_mode(half, interleaved) == kAny, H, D, B * T), (cudaStream_t)stream, p);
 }
 
 extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
@@ -591,12 +602,12 @@ extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64
   rotary_out(p.t[0], rotary_view(q_out, folded)); rotary_out(p.t[1], rotary_view(k_out, folded));
   p.t[0].w = wq; p.t[0].w_dtype = wq_dtype; p.t[0].w_sh = wq_sh;
   p.t[1].w = wk; p.t[1].w_dtype = wk_dtype; p.t[1].w_sh = wk_sh;
-  return rotary_launch(kNormTurn, dtype, half, interleaved, rotary_grid(H + Hk, D, B * T, rot_fwd_per_sm(rotary_mode(half, interleaved))), (cudaStream_t)stream, p);
+  return rotary_launch(kNormTurn, dtype, half, interleaved, rotary_grid(kNormTurn, rotary_mode(half, interleaved) == kAny, H + Hk, D, B * T), (cudaStream_t)stream, p);
 }
 
 extern "C" int64_t fox_qk_norm_rotary_partials(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D) {
   if (B <= 0 || T <= 0 || H <= 0 || Hk <= 0 || (D != 16 && D != 32 && D != 64 && D != 128)) return 1;
-  return rotary_grid(H + Hk, D, B * T, kRotBwdPerSm).ranges;
+  return rotary_grid(kNormBack, false, H + Hk, D, B * T).ranges;
 }
 
 extern "C" int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t D,
@@ -630,7 +641,7 @@ extern "C" int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64
   p.t[1].w = wk; p.t[1].w_dtype = wk_dtype; p.t[1].w_sh = wk_sh;
   p.dw_partial = dw_partial;
   p.fold = !wq_sh && !wk_sh;
-  const RotaryGrid g = rotary_grid(H + Hk, D, B * T, kRotBwdPerSm);
+  const RotaryGrid g = rotary_grid(kNormBack, false, H + Hk, D, B * T);
   cudaStream_t st = (cudaStream_t)stream;
   if (int rc = rotary_launch(kNormBack, dtype, half, interleaved, g, st, p)) return rc;
   const RotaryDwParams d = p.fold ? RotaryDwParams{dw_partial, {dwq, dwk}, {wq_dtype, wk_dtype}, {0, 0}, {1, 1}, g.ranges * g.blocks, (int)D}
