@@ -225,9 +225,8 @@ __device__ __forceinline__ void rot_exchange(const RotaryParams& p, uint16_t* sl
   for (int j = 0; j < 8; ++j) pair[j] = unpack2<kBf16>(row[rot_other(p, ch + j)]).x;
 }
 
-// grid: (ranges of per_cta tokens, blocks of heads_here heads); blockDim.x = heads_here * D / 8 up to a whole warp.  One wave of
-// CTAs with equal ranges, each in tiles of one sequence's tokens: of tiles as CTAs (16 tokens, 2.3 waves of them) the
-// norm of 2 x 8192 tokens x 32 heads of 128 took 74 us.
+// grid: (ranges of per_cta tokens, blocks of heads_here heads); blockDim.x = heads_here * D / 8 up to a whole warp.  Equal
+// ranges (rotary_grid), each in tiles of one sequence's tokens.
 template <bool kBf16, int kMode, bool kNorm, int kD>
 __global__ void __launch_bounds__(kRotThreads, rot_fwd_per_sm(kMode)) fox_rotary_fwd_kernel(const RotaryParams p) {
   constexpr int kAhead = kMode == kAny ? 2 : kRotAhead;
@@ -473,7 +472,10 @@ struct RotaryGrid {
   int blocks, heads_here, threads, ranges, per_cta, tile;
 };
 enum RotaryKind { kTurn, kNormTurn, kNormBack };
-// Heads of a token over as few CTAs of up to 256 threads as hold them, evenly; tokens over as many ranges as make one wave.  CTAs of
+// Heads of a token over as few CTAs of up to 256 threads as hold them, evenly; tokens over as many ranges as make one wave.  Forward,
+// up to four waves while ranges keep 8 tokens: SMs get uneven shares of the bandwidth, and one that is ahead takes the next range
+// (norms of 2 x 8192 tokens x 32 heads of 128: 1 wave 48.5 us, 3 45.4; 32768 tokens x 24 heads of 64 rotated only: 36.5, 4 waves 34.9).
+// Not where the angles of a range cost more (kAny: 83 us, 92), nor backward, where every range adds a share of dw (70 us, 2 waves 73).  CTAs of
 // fewer threads are more to an SM (36 heads of 64, 160 threads each: 61 -> 57 us, backward 104 -> 88), up to the threads that a kernel is
 // fastest with (24 heads of 64 rotated only, 192 threads: 4 CTAs 36.5 us, 5 37.2); where the weights' shares are added up
 // afterwards, while ranges keep 16 tokens (3000 tokens x 16 heads of 64: 8.9 us, of 6 tokens 11.2).
@@ -486,7 +488,12 @@ static RotaryGrid rotary_grid(RotaryKind kind, bool any, int64_t heads, int64_t 
   const int64_t more = by_threads < by_smem ? by_threads : by_smem;
   auto ranges = [&](int64_t per_sm) { return kSms * per_sm / blocks < 1 ? 1 : kSms * per_sm / blocks; };
   int64_t want = ranges(more > least ? more : least);
-  if (kind == kNormBack && tokens < 16 * want) want = ranges(least) > tokens / 16 ? ranges(least) : tokens / 16;
+  if (kind != kNormBack && !any) {
+    const int64_t waves = tokens / (8 * want);
+    want *= waves < 1 ? 1 : waves < 4 ? waves : 4;
+  } else if (kind == kNormBack && tokens < 16 * want) {
+    want = ranges(least) > tokens / 16 ? ranges(least) : tokens / 16;
+  }
   const int64_t per = (tokens + want - 1) / want;
   return {static_cast<int>(blocks), static_cast<int>(here), static_cast<int>(threads),
           static_cast<int>((tokens + per - 1) / per), static_cast<int>(per), static_cast<int>(per < kRotTile ? per : kRotTile)};
