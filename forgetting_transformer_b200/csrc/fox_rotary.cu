@@ -221,8 +221,17 @@ __device__ __forceinline__ void rot_exchange(const RotaryParams& p, uint16_t* sl
   *reinterpret_cast<uint4*>(slot + lane * 8) = v;
   __syncwarp();
   const uint16_t* row = slot + (lane & ~(lanes - 1)) * 8;
+  if (p.half & 1) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) pair[j] = unpack2<kBf16>(row[rot_other(p, ch + j)]).x;
+    for (int j = 0; j < 8; ++j) pair[j] = unpack2<kBf16>(row[rot_other(p, ch + j)]).x;
+  } else {   // (two neighbours' others are neighbours: norms of 16384 tokens x 32 heads of 128, half 22, 70 us, half 21 84)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = unpack2<kBf16>(*reinterpret_cast<const uint32_t*>(row + rot_other(p, ch + 2 * j)));
+      pair[2 * j] = f.x;
+      pair[2 * j + 1] = f.y;
+    }
+  }
 }
 
 // grid: (ranges of per_cta tokens, blocks of heads_here heads); blockDim.x = heads_here * D / 8 up to a whole warp.  Equal

@@ -413,3 +413,18 @@ def test_second_derivatives():
         torch.autograd.grad(g[0].float().sum(), [q])
     out = fox.qk_norm_rotary(q, k, w, w, inv_freq)
     assert not torch.autograd.grad(out[0].float().sum(), [q])[0].requires_grad
+
+
+@pytest.mark.parametrize("T,H,D", [(120001, 3, 16), (30011, 32, 64)])
+def test_many_tokens(T, H, D):
+    """Several ranges of tokens for every place of a CTA on the GPU, the last of them short: every token is turned, and normed, once."""
+    x = data(T, 1, T, H, D, dtype=torch.bfloat16)
+    inv_freq, _ = fox.rotary_frequencies(D, device="cuda")
+    a = angles64(torch.arange(T, device="cuda"), inv_freq)[None, :, None]
+    w = torch.full((D,), 0.75, device="cuda")
+    y = fox.rotary_embedding(x, inv_freq)
+    q, k = fox.qk_norm_rotary(x, x, w, w, inv_freq)
+    n = norm64(x.double(), 0.75, 1e-5)
+    for got, src, slack in ((y, x.double(), 2 ** -20), (q, n, 2 ** -19), (k, n, 2 ** -19)):
+        ref = turn64(src, a, False)
+        assert ((got.double() - ref).abs() <= 2 ** -8 * ref.abs() + slack * reach(src, D // 2, False)).all()
