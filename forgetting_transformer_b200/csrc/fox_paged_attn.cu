@@ -19,15 +19,16 @@
 // what the cache's length costs), and the parts' sums shift their maxima when they are joined.
 //
 // One lane of a warp asks for a tile (TMA, 128-byte swizzle; the gates each lane by 16 bytes for itself) into a ring of
-// kStages tiles that is the warp's own: no warp waits for another.  (Each lane copying by cp.async what it feeds to the matrix
+// kStages tiles (of small ones, pairs) that is the warp's own: no warp waits for another.  (Each lane copying by cp.async what it feeds to the matrix
 // instructions itself needed no barrier, but its 300 instructions a tile queued for shared memory: 3.6 TB/s.)
 // mma.sync m16n8k16 (the two products are 8 query rows at most; the kernel is bound by memory, with a tensor pipe mostly idle):
 //   S (16 x 8 keys) = Q K^T, twice, rows 0-7 the unit's query heads.  Lane (x = lane / 4, c = lane % 4) gives 16-byte pieces
-//     2 c and 2 c + 1 of a key's row; which channels stand at which k of an instruction does not matter as long as Q stands the
+//     2 c and 2 c + 1 of a key's row (of each 64 channels; of 32, piece c; of 16, half a piece); which channels stand at which k of an instruction does not matter as long as Q stands the
 //     same way.  The two key columns that a lane gets of each S are keys 4 c .. 4 c + 3 of the tile.
 //   O (16 x D) += P V.  The registers of S are those of P.  P is rounded to 16 bits, and what the rounding leaves stands in
 //     rows 8-15, which would be idle: the sum of the two halves of O has P to 2^-16 (fp16: 2^-21).
-// Head dims 16 and 32 go through the 64-column tiles, filled with zeros by the copies.
+// Head dims 16 and 32, whose tiles are small, are bound by a tile's chain of instructions: a warp takes two tiles together, through
+// boxes as wide as they are (16 requests of 1000 to 9000 keys x 16 heads of 32, 126 MB: one tile, filled up to 64 columns, 38 us; two 32).
 //
 // Tiles never leave a page (pages are 16 keys at least).  Rows behind the last key may hold anything: their logits are
 // replaced, their values set to zero.  A table entry outside the pool is not read: its keys take no part.
@@ -42,7 +43,7 @@ constexpr int kPagGrid = kSms;
 // Warps of a CTA, each with two tiles asked for: some 110 and 140 KB in flight on an SM.  More is slower, since SMs then get more
 // uneven shares of the bandwidth (24 x 65536 keys of 64: 12 warps x 2 tiles 70.5 us, 16 x 3 76; 32 x 2048 x 16 heads of 128: 8 x 2
 // 91, 8 x 3 98, 10 x 2 94), fewer warps too (8 x 4 88).  Head dims 16 and 32 are bound by what a tile takes a warp, not by its
-// bytes: 16 warps (16 requests of 1000 to 9000 keys x 16 heads of 32: 12 warps 45 us, 16 38).
+// bytes: 16 warps (16 requests of 1000 to 9000 keys x 16 heads of 32: 12 warps 35 us, 16 32).
 __host__ __device__ constexpr int pag_warps(int64_t D) { return D == 128 ? 8 : D == 64 ? 12 : 16; }
 constexpr int kPagTile = 16;
 constexpr int kPagRows = 8;          // query heads of a unit
@@ -132,22 +133,35 @@ __device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint2 lds_v2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 template <int D>
 struct PagedTile {
-  static constexpr int kHalves = D == 128 ? 2 : 1;            // boxes of 16 keys x 64 columns
-  static constexpr int kBox = kPagTile * 128;
-  static constexpr int kStage = 2 * kHalves * kBox;           // keys, values
-  static constexpr int kGates = kPagRows * kPagTile * 4;
+  static constexpr int kHalves = D == 128 ? 2 : 1;            // boxes of 16 keys x 64 columns, or of all columns
+  static constexpr int kRow = D < 64 ? D * 2 : 128;           // bytes of a row in a box, over which the copy's swizzle goes
+  static constexpr int kBox = kPagTile * kRow;
+  static constexpr int kTile = 2 * kHalves * kBox;            // keys, values
+  static constexpr int kSub = D < 64 ? 2 : 1;                 // tiles that a warp takes together
+  static constexpr int kStage = kSub * kTile;
+  static constexpr int kGates = kSub * kPagRows * kPagTile * 4;
   static constexpr int kCols = D / 8;                         // n of the second product
   static constexpr int kStages = 2;
   static constexpr int kWarps = pag_warps(D), kThreads = kWarps * 32;
   static constexpr int kParts = kWarps * kStages * (kStage + kGates);   // where the warps' parts begin: (warps, 2, rows, D + 4)
   static constexpr int kSmem = kParts + kWarps * 2 * kPagRows * (D + 4) * 4 + 1024;   // (boxes begin at multiples of 1024 bytes)
+  // where the swizzle has put 16-byte piece `piece` of a key's row
+  static __device__ __forceinline__ uint32_t at(uint32_t key, uint32_t piece) {
+    return key * kRow + (piece ^ (D < 32 ? (key >> 2) & 1 : D < 64 ? (key >> 1) & 3 : key & 7)) * 16;
+  }
 };
 
-// What a stage's tile is: written by lane 0, read by the warp.
+// What a stage's tiles are: written by lane 0, read by the warp.
 struct PagedItem {
-  int r, h0, valid, flags;   // first query head; keys of the tile that count; kItemFirst ... below, and the heads from bit 8 on
+  int r, h0, valid, flags;   // first query head; keys of the tiles that count, 8 bits for each; kItemFirst ... below, and the heads from bit 8 on
 };
 enum { kItemFirst = 1, kItemLast = 2, kItemWhole = 4, kItemSecond = 8 };   // of its part; a unit's only part; workspace place 1
 
@@ -159,7 +173,7 @@ template <bool kBf16, int D>
 __global__ void __launch_bounds__(PagedTile<D>::kThreads, 1)
 fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v) {
   using Tile = PagedTile<D>;
-  constexpr int kStages = Tile::kStages, kThreads = Tile::kThreads, kWarps = Tile::kWarps;
+  constexpr int kStages = Tile::kStages, kThreads = Tile::kThreads, kWarps = Tile::kWarps, kSub = Tile::kSub;
   extern __shared__ __align__(1024) char pag_smem[];
   __shared__ uint64_t s_full[kWarps][kStages];
   __shared__ int s_abort;
@@ -300,44 +314,64 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   const int x = lane >> 2, c = lane & 3;
   // (rows of gates that no head fills: finite)
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) *reinterpret_cast<float4*>(ring_g + s * (Tile::kGates / 4) + lane * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < kStages * kSub; ++s) *reinterpret_cast<float4*>(ring_g + s * (kPagRows * kPagTile) + lane * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
   const uint32_t ring_u32 = smem_u32(ring), gates_u32 = smem_u32(ring_g) + lane * 16;
   int page_r = -1, page_base = 0, page_ids = -1;   // 32 entries of a request's table row, one to a lane
 
   int ask_stage = 0;
   int pending = 0;   // tiles asked for and not yet used
-  auto ask = [&]() {   // the next tile
+  auto ask = [&]() {   // the next kSub tiles
     if (at < part_lo) {
       cp_async_commit();
       return;
     }
-    const int key0 = at * kPagTile, j = key0 >> p.page_log2, row0 = key0 & ((1 << p.page_log2) - 1);
-    if (r != page_r || j < page_base || j >= page_base + 32) {
-      page_r = r;
-      page_base = j < 31 ? 0 : j - 31;   // (the walk goes to the left)
-      const int e = page_base + lane;
-      page_ids = static_cast<int64_t>(e) << p.page_log2 < length ? p.table[r * p.table_ld + e] : -1;
+    int id[kSub], row0[kSub], valid = 0, loads = 0;
+#pragma unroll
+    for (int s = kSub - 1; s >= 0; --s) {   // (the walk goes to the left)
+      id[s] = -1;
+      row0[s] = 0;
+      if (at < part_lo) continue;
+      const int key0 = at * kPagTile, j = key0 >> p.page_log2;
+      row0[s] = key0 & ((1 << p.page_log2) - 1);
+      if (r != page_r || j < page_base || j >= page_base + 32) {
+        page_r = r;
+        page_base = j < 31 ? 0 : j - 31;
+        const int e = page_base + lane;
+        page_ids = static_cast<int64_t>(e) << p.page_log2 < length ? p.table[r * p.table_ld + e] : -1;
+      }
+      const int page = __shfl_sync(0xffffffffu, page_ids, j - page_base);
+      if (page >= 0 && page < p.n_pages) {
+        id[s] = page;
+        valid |= min(length - key0, kPagTile) << (8 * s);
+        ++loads;
+      }
+      --at;
     }
-    const int id = __shfl_sync(0xffffffffu, page_ids, j - page_base);
-    const bool there = id >= 0 && id < p.n_pages, last = at == part_lo;
+    const bool last = at < part_lo;
     uint64_t* const bar = &s_full[warp][ask_stage];
     if (lane == 0) {
-      s_item[warp][ask_stage] = {r, h0, there ? min(length - key0, kPagTile) : 0, flags | (last ? kItemLast : 0)};
-      if (there) {
-        mbar_expect_tx(bar, Tile::kStage);
-        const uint32_t to = ring_u32 + ask_stage * Tile::kStage;
-        tma_load_5d(to, &map_k, bar, row0, kh, id);
-        tma_load_5d(to + Tile::kStage / 2, &map_v, bar, row0, kh, id);
+      s_item[warp][ask_stage] = {r, h0, valid, flags | (last ? kItemLast : 0)};
+      if (loads) {
+        mbar_expect_tx(bar, loads * Tile::kTile);
+#pragma unroll
+        for (int s = 0; s < kSub; ++s) {
+          const uint32_t to = ring_u32 + ask_stage * Tile::kStage + s * Tile::kTile;
+          if (id[s] < 0) continue;
+          tma_load_5d(to, &map_k, bar, row0[s], kh, id[s]);
+          tma_load_5d(to + Tile::kTile / 2, &map_v, bar, row0[s], kh, id[s]);
+        }
       } else {
         mbar_arrive(bar);
       }
     }
-    if (there && x < heads) cp_async_16(gates_u32 + ask_stage * Tile::kGates, p.gates + id * p.g_sp + (h0 + x) * p.g_sh + row0 + 4 * c);
+#pragma unroll
+    for (int s = 0; s < kSub; ++s)
+      if (id[s] >= 0 && x < heads)
+        cp_async_16(gates_u32 + ask_stage * Tile::kGates + s * (kPagRows * kPagTile * 4), p.gates + id[s] * p.g_sp + (h0 + x) * p.g_sh + row0[s] + 4 * c);
     cp_async_commit();
-    if ((flags & kItemFirst) && x < heads) touch(p.q + r * p.q_sr + (h0 + x) * p.q_sh + (D == 16 ? c * 4 : D == 32 ? c * 8 : c * 16));
+    if ((flags & kItemFirst) && x < heads) touch(p.q + r * p.q_sr + (h0 + x) * p.q_sh + (D < 32 ? c * 4 : D < 64 ? c * 8 : c * 16));
     flags &= ~kItemFirst;
     ++pending;
-    --at;
     if (last && left > 0) {   // the next unit
       place = 0;
       if (++unit == p.units) {
@@ -356,12 +390,14 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
   for (int s = 0; s < kStages - 1; ++s) ask();
 
   constexpr float kShift = kBf16 ? 0.f : 12.f;   // fp16: weights up to 2^12, so that small ones keep their bits
-  // a lane's first piece of keys 4 (x / 2) + x % 2 in a box, where the swizzle has put it; the next piece: ^ 16; 2 keys on: + 256, ^ 32
-  const uint32_t key_a = 4 * (x >> 1) + (x & 1), k_off = key_a * 128 + ((2 * c) ^ (key_a & 7)) * 16;
+  // a lane's pieces of keys 4 (x / 2) + x % 2 and 2 on in a box: from 64 columns on, 2 c and (^ 16) 2 c + 1; of 32 columns, c; of 16,
+  // half of one
+  const uint32_t key_a = 4 * (x >> 1) + (x & 1), piece = D < 32 ? c >> 1 : D < 64 ? c : 2 * c;
+  const uint32_t k_off = Tile::at(key_a, piece) + (D < 32 ? (c & 1) * 8 : 0), k_off2 = Tile::at(key_a + 2, piece) + (D < 32 ? (c & 1) * 8 : 0);
   // the row of the values whose address a lane gives: keys 4 (j / 2) + j % 2, in matrices 1 and 3 2 on; in 2 and 3 the next 8 columns
-  const uint32_t key_v = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * ((lane >> 3) & 1),
-                 v_off = key_v * 128 + ((static_cast<uint32_t>(lane) >> 4) ^ (key_v & 7)) * 16;
-  uint4 qf[2 * Tile::kHalves];   // channels (2 c + s) 8 .. of each half
+  const uint32_t key_v = 4 * ((lane & 7) >> 1) + (lane & 1) + 2 * ((lane >> 3) & 1), v_off = Tile::at(key_v, static_cast<uint32_t>(lane) >> 4);
+  constexpr int kPieces = D < 64 ? 1 : 2 * Tile::kHalves;
+  uint4 qf[kPieces];   // the channels of a lane's pieces
   float o[Tile::kCols][4], m = -INFINITY, l = 0.f, carry = 0.f;
   int stage = 0;
   uint32_t parity = 0;
@@ -376,10 +412,19 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
     const uint32_t tile = ring_u32 + stage * Tile::kStage;
     const bool row = x < item.flags >> 8;   // a row of the unit
     if (item.flags & kItemFirst) {
-      const uint16_t* qp = p.q + item.r * p.q_sr + (item.h0 + x) * p.q_sh + c * 16;
+      constexpr int kOwn = D < 32 ? 4 : D < 64 ? 8 : 16;   // channels of a lane in 64, or in all
+      const uint16_t* qp = p.q + item.r * p.q_sr + (item.h0 + x) * p.q_sh + c * kOwn;
 #pragma unroll
-      for (int s = 0; s < 2 * Tile::kHalves; ++s)
-        qf[s] = row && (s & 1) * 8 + c * 16 < D ? *reinterpret_cast<const uint4*>(qp + (s >> 1) * 64 + (s & 1) * 8) : make_uint4(0u, 0u, 0u, 0u);
+      for (int s = 0; s < kPieces; ++s) {
+        qf[s] = make_uint4(0u, 0u, 0u, 0u);
+        if constexpr (D < 32) {
+          const uint2 v = row ? *reinterpret_cast<const uint2*>(qp) : make_uint2(0u, 0u);
+          qf[s].x = v.x;
+          qf[s].y = v.y;
+        } else if (row) {
+          qf[s] = *reinterpret_cast<const uint4*>(qp + (s >> 1) * 64 + (s & 1) * 8);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < Tile::kCols; ++j)
 #pragma unroll
@@ -387,49 +432,81 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
       m = -INFINITY;
       l = carry = 0.f;
     }
-    // ---- gates: sums behind each of the lane's four keys, inside the part
-    float bias[4];
-    {
-      const float4 gv = *reinterpret_cast<const float4*>(ring_g + stage * (Tile::kGates / 4) + lane * 4);
-      float g[4] = {gv.x, gv.y, gv.z, gv.w};
-      if (item.valid < kPagTile) {
+    int valid[kSub];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (4 * c + i >= item.valid) g[i] = 0.f;
+    for (int s = 0; s < kSub; ++s) valid[s] = kSub == 1 ? item.valid : item.valid >> (8 * s) & 255;
+    // ---- gates: sums behind each of the lane's four keys, inside the part
+    float bias[kSub][4];
+    {
+      float own[kSub][3], behind[kSub], y[kSub];   // behind: of this lane and those to its right
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) {
+        const float4 gv = *reinterpret_cast<const float4*>(ring_g + (stage * kSub + s) * (kPagRows * kPagTile) + lane * 4);
+        float g[4] = {gv.x, gv.y, gv.z, gv.w};
+        if (valid[s] < kPagTile) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (4 * c + i >= valid[s]) g[i] = 0.f;
+        }
+        own[s][2] = g[3];
+        own[s][1] = g[3] + g[2];
+        own[s][0] = own[s][1] + g[1];
+        behind[s] = own[s][0] + g[0];
       }
-      const float own2 = g[3], own1 = g[3] + g[2], own0 = own1 + g[1];
-      float behind = own0 + g[0];   // of this lane and those to its right
-      float y = __shfl_down_sync(0xffffffffu, behind, 1, 4);
-      if (c < 3) behind += y;
-      y = __shfl_down_sync(0xffffffffu, behind, 2, 4);
-      if (c < 2) behind += y;
-      y = __shfl_down_sync(0xffffffffu, behind, 1, 4);   // (not behind - sum: a gate of minus infinity cannot be taken off again)
-      const float right = c < 3 ? carry + y : carry;
-      bias[0] = (right + own0) * kPagLog2e;
-      bias[1] = (right + own1) * kPagLog2e;
-      bias[2] = (right + own2) * kPagLog2e;
-      bias[3] = right * kPagLog2e;
-      carry += __shfl_sync(0xffffffffu, behind, 0, 4);
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) y[s] = __shfl_down_sync(0xffffffffu, behind[s], 1, 4);
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) behind[s] += c < 3 ? y[s] : 0.f;
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) y[s] = __shfl_down_sync(0xffffffffu, behind[s], 2, 4);
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) behind[s] += c < 2 ? y[s] : 0.f;
+#pragma unroll
+      for (int s = 0; s < kSub; ++s) y[s] = __shfl_down_sync(0xffffffffu, behind[s], 1, 4);   // (not behind - sum: a gate of minus
+                                                                                             // infinity cannot be taken off again)
+#pragma unroll
+      for (int s = kSub - 1; s >= 0; --s) {
+        const float right = c < 3 ? carry + y[s] : carry;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) bias[s][i] = (right + own[s][i]) * kPagLog2e;
+        bias[s][3] = right * kPagLog2e;
+        carry += __shfl_sync(0xffffffffu, behind[s], 0, 4);
+      }
     }
     // ---- S
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    float u[kSub][4];
 #pragma unroll
-    for (int s = 0; s < 2 * Tile::kHalves; ++s) {
-      const uint32_t at_k = tile + (s >> 1) * Tile::kBox;
-      const uint4 ka = lds_v4(at_k + (k_off ^ ((s & 1) * 16))), kb = lds_v4(at_k + ((k_off + 256) ^ (32 + (s & 1) * 16)));
-      mma_16816<kBf16>(s0, qf[s].x, 0u, qf[s].y, 0u, ka.x, ka.y);
-      mma_16816<kBf16>(s1, qf[s].x, 0u, qf[s].y, 0u, kb.x, kb.y);
-      mma_16816<kBf16>(s0, qf[s].z, 0u, qf[s].w, 0u, ka.z, ka.w);
-      mma_16816<kBf16>(s1, qf[s].z, 0u, qf[s].w, 0u, kb.z, kb.w);
-    }
-    float u[4] = {fmaf(s0[0], p.qk_scale, bias[0]), fmaf(s0[1], p.qk_scale, bias[1]), fmaf(s1[0], p.qk_scale, bias[2]),
-                  fmaf(s1[1], p.qk_scale, bias[3])};
-    if (item.valid < kPagTile) {
+    for (int s = 0; s < kSub; ++s) {
+      float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint32_t tile_k = tile + s * Tile::kTile;
+      if constexpr (D < 32) {
+        const uint2 ka = lds_v2(tile_k + k_off), kb = lds_v2(tile_k + k_off2);
+        mma_16816<kBf16>(s0, qf[0].x, 0u, qf[0].y, 0u, ka.x, ka.y);
+        mma_16816<kBf16>(s1, qf[0].x, 0u, qf[0].y, 0u, kb.x, kb.y);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (4 * c + i >= item.valid) u[i] = -INFINITY;
+        for (int e = 0; e < kPieces; ++e) {
+          const uint32_t at_k = tile_k + (e >> 1) * Tile::kBox;
+          const uint4 ka = lds_v4(at_k + (k_off ^ ((e & 1) * 16))), kb = lds_v4(at_k + (k_off2 ^ ((e & 1) * 16)));
+          mma_16816<kBf16>(s0, qf[e].x, 0u, qf[e].y, 0u, ka.x, ka.y);
+          mma_16816<kBf16>(s1, qf[e].x, 0u, qf[e].y, 0u, kb.x, kb.y);
+          mma_16816<kBf16>(s0, qf[e].z, 0u, qf[e].w, 0u, ka.z, ka.w);
+          mma_16816<kBf16>(s1, qf[e].z, 0u, qf[e].w, 0u, kb.z, kb.w);
+        }
+      }
+      u[s][0] = fmaf(s0[0], p.qk_scale, bias[s][0]);
+      u[s][1] = fmaf(s0[1], p.qk_scale, bias[s][1]);
+      u[s][2] = fmaf(s1[0], p.qk_scale, bias[s][2]);
+      u[s][3] = fmaf(s1[1], p.qk_scale, bias[s][3]);
+      if (valid[s] < kPagTile) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * c + i >= valid[s]) u[s][i] = -INFINITY;
+      }
     }
-    float mx = fmaxf(fmax3(u[0], u[1], u[2]), fmaxf(u[3], m));
+    float mx = m;
+#pragma unroll
+    for (int s = 0; s < kSub; ++s) mx = fmaxf(fmax3(u[s][0], u[s][1], u[s][2]), fmaxf(u[s][3], mx));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m)) {   // (NaN logits: no new maximum, and NaN weights)
@@ -442,35 +519,38 @@ fox_paged_attn_kernel(const PagedParams p, const __grid_constant__ CUtensorMap m
       m = mx;
     }
     const float ref = m == -INFINITY ? 0.f : m - kShift;
-    // ---- P, its 16-bit values and what they leave
-    float w[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = fast_exp2(u[i] - ref);
-    l += (w[0] + w[1]) + (w[2] + w[3]);
-    const uint32_t hi0 = pack2<kBf16>(w[0], w[1]), hi1 = pack2<kBf16>(w[2], w[3]);
-    const float2 r0 = unpack2<kBf16>(hi0), r1 = unpack2<kBf16>(hi1);
-    const uint32_t lo0 = pack2<kBf16>(w[0] - r0.x, w[1] - r0.y), lo1 = pack2<kBf16>(w[2] - r1.x, w[3] - r1.y);
-    // ---- O
-    const uint32_t tile_v = tile + Tile::kHalves * Tile::kBox;
-    const bool whole = item.valid == kPagTile;
-    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;   // of keys 4 c, 4 c + 1; of the next two
-    if (!whole) {
-      const int n = item.valid - 4 * c;
-      keep0 = n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u;
-      keep1 = n >= 4 ? 0xffffffffu : n == 3 ? 0xffffu : 0u;
-    }
+    for (int s = 0; s < kSub; ++s) {
+      // ---- P, its 16-bit values and what they leave
+      float w[4];
 #pragma unroll
-    for (int j = 0; j < Tile::kCols; j += 2) {
-      uint32_t v[4];
-      ldmatrix_x4_trans(tile_v + (j >> 3) * Tile::kBox + (v_off ^ ((j & 7) * 16)), v);
-      if (!whole) {   // (a row behind the last key may hold anything, and zero times NaN is NaN)
-        v[0] &= keep0;
-        v[1] &= keep1;
-        v[2] &= keep0;
-        v[3] &= keep1;
+      for (int i = 0; i < 4; ++i) w[i] = fast_exp2(u[s][i] - ref);
+      l += (w[0] + w[1]) + (w[2] + w[3]);
+      const uint32_t hi0 = pack2<kBf16>(w[0], w[1]), hi1 = pack2<kBf16>(w[2], w[3]);
+      const float2 r0 = unpack2<kBf16>(hi0), r1 = unpack2<kBf16>(hi1);
+      const uint32_t lo0 = pack2<kBf16>(w[0] - r0.x, w[1] - r0.y), lo1 = pack2<kBf16>(w[2] - r1.x, w[3] - r1.y);
+      // ---- O
+      const uint32_t tile_v = tile + s * Tile::kTile + Tile::kHalves * Tile::kBox;
+      const bool whole = valid[s] == kPagTile;
+      uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;   // of keys 4 c, 4 c + 1; of the next two
+      if (!whole) {
+        const int n = valid[s] - 4 * c;
+        keep0 = n >= 2 ? 0xffffffffu : n == 1 ? 0xffffu : 0u;
+        keep1 = n >= 4 ? 0xffffffffu : n == 3 ? 0xffffu : 0u;
       }
-      mma_16816<kBf16>(o[j], hi0, lo0, hi1, lo1, v[0], v[1]);
-      mma_16816<kBf16>(o[j + 1], hi0, lo0, hi1, lo1, v[2], v[3]);
+#pragma unroll
+      for (int j = 0; j < Tile::kCols; j += 2) {
+        uint32_t v[4];
+        ldmatrix_x4_trans(tile_v + (j >> 3) * Tile::kBox + (v_off ^ ((j & 7) * 16)), v);
+        if (!whole) {   // (a row behind the last key may hold anything, and zero times NaN is NaN)
+          v[0] &= keep0;
+          v[1] &= keep1;
+          v[2] &= keep0;
+          v[3] &= keep1;
+        }
+        mma_16816<kBf16>(o[j], hi0, lo0, hi1, lo1, v[0], v[1]);
+        mma_16816<kBf16>(o[j + 1], hi0, lo0, hi1, lo1, v[2], v[3]);
+      }
     }
     if (item.flags & kItemLast) {
       float ls = l + __shfl_xor_sync(0xffffffffu, l, 1);
@@ -741,15 +821,16 @@ __global__ void __launch_bounds__(kJoinThreads) fox_paged_join_kernel(const Page
   if (!waited) wait_for_kernel_in_front();   // (this grid's end has to mean the first kernel's)
 }
 
-// (64 columns, rows of a page, halves, heads, pages); a head dim below 64: the columns behind it are filled with zeros
+// (64 columns or all, rows of a page, halves, heads, pages)
 static int make_paged_tmap(CUtensorMap* out, const fox_tensor4* t, bool bf16, int64_t P, int64_t heads, int64_t page, int64_t D) {
   EncodeTiledFn fn = get_encode_tiled();
   if (!fn) return FOX_ERR_DRIVER;
   const cuuint64_t dims[5] = {(cuuint64_t)(D < 64 ? D : 64), (cuuint64_t)page, (cuuint64_t)(D == 128 ? 2 : 1), (cuuint64_t)heads, (cuuint64_t)P};
   const cuuint64_t strides[4] = {(cuuint64_t)t->st * 2, 128, (cuuint64_t)t->sh * 2, (cuuint64_t)t->sb * 2};
-  const cuuint32_t box[5] = {64, kPagTile, (cuuint32_t)(D == 128 ? 2 : 1), 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+  const cuuint32_t box[5] = {(cuuint32_t)(D < 64 ? D : 64), kPagTile, (cuuint32_t)(D == 128 ? 2 : 1), 1, 1}, ones[5] = {1, 1, 1, 1, 1};
+  const CUtensorMapSwizzle swizzle = D < 32 ? CU_TENSOR_MAP_SWIZZLE_32B : D < 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
   return fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, t->ptr, dims, strides, box, ones,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
              ? FOX_OK
              : FOX_ERR_TENSORMAP;
