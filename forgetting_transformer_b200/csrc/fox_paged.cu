@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kTabThreads) fox_page_tables_kernel(const Tabl
   __shared__ int s_served;
   if (threadIdx.x == 0) s_served = s_starts[0] = 0;
   wait_for_kernel_in_front();
+  if (!place) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (the placing kernel, which waits for this one's end)
   const int free_before = max(0, min(*p.num_free, p.n_free_max));
   const int64_t page_less_1 = (1 << p.page_log2) - 1;
   const bool staged = p.R <= kTabThreads;   // all requests in shared memory

@@ -744,6 +744,7 @@ __global__ void __launch_bounds__(kJoinThreads) fox_paged_join_kernel(const Page
     if (!waited) {
       wait_for_kernel_in_front();
       waited = true;
+      asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // (what comes behind is launched meanwhile: 0.7 us)
     }
     float4 ahead[kAhead];
 #pragma unroll
