@@ -199,10 +199,12 @@ __global__ void __launch_bounds__(kTabThreads) fox_release_pages_kernel(const Re
 
 // ------------------------------------------------------------------- rows
 // Bound by HBM: each row is read once and written once.  A CTA takes a tile of tokens; a thread holds one 16-byte piece of a
-// token's keys or values and goes through the tile with it, kUpdAhead tokens' loads in front of their stores.  The gates of a
+// token's keys or values and goes through the tile with it, kAhead tokens' loads in front of their stores (8 where an
+// SM has 16 tiles or more: 30000 tokens x 24 heads of 64 59.9 -> 57.5 us; else 4, which take fewer registers: 5000 tokens x 16 heads of
+// 128 16.0 -> 15.4, 2000 7.9 -> 6.0).  The gates of a
 // tile go with one token to a lane, so that tokens behind one another in a page are written side by side.
-// (30000 tokens x 24 heads of 64, tiles of 32 / 16 / 8 tokens: 64, 61, 60 us; 16 heads of 128: 81, 77, 74.)
-constexpr int kUpdThreads = 256, kUpdTile = 8, kUpdAhead = 4;
+// (30000 tokens x 24 heads of 64, tiles of 32 / 16 / 8 tokens with 4 ahead: 64, 61, 60 us; 16 heads of 128: 81, 77, 74.)
+constexpr int kUpdThreads = 256, kUpdTile = 8;   // threads: at most
 
 struct UpdateParams {
   const uint16_t *k, *v;
@@ -231,6 +233,7 @@ __device__ __forceinline__ float upd_gate(const UpdateParams& p, int64_t i) {
   return fminf(x, 0.f) - log1pf(expf(-fabsf(x)));
 }
 
+template <int kAhead>
 __global__ void __launch_bounds__(kUpdThreads) fox_paged_update_kernel(const UpdateParams p) {
   __shared__ int64_t s_page[kUpdTile];
   __shared__ int s_row[kUpdTile];
@@ -245,23 +248,23 @@ __global__ void __launch_bounds__(kUpdThreads) fox_paged_update_kernel(const Upd
   }
   __syncthreads();
   const int pieces = p.Hk * p.lanes;
-  for (int c = threadIdx.x; c < 2 * pieces; c += kUpdThreads) {
+  for (int c = threadIdx.x; c < 2 * pieces; c += blockDim.x) {
     const bool is_v = c >= pieces;
     const int i = is_v ? c - pieces : c, h = i / p.lanes, sub = i - h * p.lanes;
     const uint16_t* from = (is_v ? p.v + h * p.v_sh + t0 * p.v_st : p.k + h * p.k_sh + t0 * p.k_st) + sub * 8;
     uint16_t* to = (is_v ? p.v_pages + h * p.v_sk : p.k_pages + h * p.k_sk) + sub * 8;
     const int64_t st = is_v ? p.v_st : p.k_st, sp = is_v ? p.v_sp : p.k_sp, sr = is_v ? p.v_sr : p.k_sr;
-    for (int u0 = 0; u0 < n; u0 += kUpdAhead) {
-      uint4 x[kUpdAhead];
+    for (int u0 = 0; u0 < n; u0 += kAhead) {
+      uint4 x[kAhead];
 #pragma unroll
-      for (int u = 0; u < kUpdAhead; ++u)
+      for (int u = 0; u < kAhead; ++u)
         if (u0 + u < n) x[u] = ld_v4_here(reinterpret_cast<const uint4*>(from + (u0 + u) * st));
 #pragma unroll
-      for (int u = 0; u < kUpdAhead; ++u)
+      for (int u = 0; u < kAhead; ++u)
         if (u0 + u < n && s_page[u0 + u] >= 0) *reinterpret_cast<uint4*>(to + s_page[u0 + u] * sp + s_row[u0 + u] * sr) = x[u];
     }
   }
-  for (int i = threadIdx.x; i < p.H * kUpdTile; i += kUpdThreads) {
+  for (int i = threadIdx.x; i < p.H * kUpdTile; i += blockDim.x) {
     const int u = i & (kUpdTile - 1), h = i / kUpdTile;
     if (u < n && s_page[u] >= 0) p.gate_pages[s_page[u] * p.g_sp + h * p.g_sk + s_row[u]] = upd_gate(p, (t0 + u) * p.g_st + h * p.g_sh);
   }
@@ -329,9 +332,14 @@ extern "C" int fox_paged_update(int device, void* stream, int64_t T, int64_t H, 
   if (cudaSetDevice(device) != cudaSuccess) return FOX_ERR_DEVICE;
   // a tile of 8 tokens, fewer where those are fewer than four CTAs to an SM
   const int64_t fit = (T + kSms * 4 - 1) / (kSms * 4), tile = fit < kUpdTile ? fit : kUpdTile;
+  // threads: a token's pieces over as few turns as 256 take, evenly; 128 at least
+  const int64_t pieces = 2 * Hk * (D / 8), turns = (pieces + kUpdThreads - 1) / kUpdThreads, even = ((pieces + turns - 1) / turns + 31) / 32 * 32;
+  const unsigned threads = even < 128 ? 128 : (unsigned)even;
   const UpdateParams p{(const uint16_t*)k, (const uint16_t*)v, k_st, k_sh, v_st, v_sh, gates, g_st, g_sh, gate_kind,
                        (uint16_t*)k_pages->ptr, (uint16_t*)v_pages->ptr, k_pages->sb, k_pages->sh, k_pages->st, v_pages->sb,
                        v_pages->sh, v_pages->st, gate_pages, gp_sp, gp_sh, slots, slots_64, T, n_pages * page, (int)H, (int)Hk,
                        (int)(D / 8), (int)tile, log2_of(page)};
-  return launch_behind(fox_paged_update_kernel, dim3((unsigned)((T + tile - 1) / tile)), kUpdThreads, 0, (cudaStream_t)stream, p);
+  const dim3 grid((unsigned)((T + tile - 1) / tile));
+  if (grid.x >= 16 * kSms) return launch_behind(fox_paged_update_kernel<kUpdTile>, grid, threads, 0, (cudaStream_t)stream, p);
+  return launch_behind(fox_paged_update_kernel<kUpdTile / 2>, grid, threads, 0, (cudaStream_t)stream, p);
 }
