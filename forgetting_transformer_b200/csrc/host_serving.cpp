@@ -338,6 +338,12 @@ void check_int32(const Tensor& t, int64_t dims, const char* what) {
 }
 int64_t table_ld(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride(0); }
 
+// The paged operators write in place and make their results outside the dispatcher: a trace would hold the results as constants
+// and none of the writes.  They have no autograd functions that could be recorded instead.
+void not_traced(const char* what) {
+  if (tracing()) raise_fox(std::string(what) + " cannot be traced: its results would be constants of the trace, and its writes lost");
+}
+
 struct Pool {   // the pages of one layer
   Tensor k, v, gates;
   int64_t P = 0, Hk = 0, H = 0, page = 0, D = 0;
@@ -486,6 +492,7 @@ FOX_PY(py_qk_norm_rotary_backward) {
 // -> (lengths, num_free, starts, granted, requests, positions, slots)
 FOX_PY(py_page_tables) {
   HANDLE_TH_ERRORS
+  not_traced("page_tables");
   const Tensor lengths = unpack(args[0], "lengths"), fresh = unpack(args[1], "new_tokens"), table = unpack(args[2], "block_table"),
                pages = unpack(args[3], "free_pages"), num_free = unpack(args[4], "num_free");
   const int64_t page = integer(args[5], "page_size"), T = integer(args[6], "max_tokens");
@@ -541,6 +548,7 @@ FOX_PY(py_page_tables) {
 // (lengths, keep, block_table, free_pages, num_free, page_size), in place
 FOX_PY(py_release_pages) {
   HANDLE_TH_ERRORS
+  not_traced("release_pages");
   const Tensor lengths = unpack(args[0], "lengths"), keep = unpack(args[1], "keep"), table = unpack(args[2], "block_table"),
                pages = unpack(args[3], "free_pages"), num_free = unpack(args[4], "num_free");
   const int64_t page = integer(args[5], "page_size");
@@ -577,6 +585,7 @@ FOX_PY(py_release_pages) {
 // (k_pages, v_pages, gate_pages, k, v, gates, slots, gate_is_logit), in place
 FOX_PY(py_paged_update) {
   HANDLE_TH_ERRORS
+  not_traced("paged_update");
   const Tensor kp = unpack(args[0], "k_pages"), vp = unpack(args[1], "v_pages"), gp = unpack(args[2], "gate_pages");
   const Tensor k_in = unpack(args[3], "k"), v_in = unpack(args[4], "v"), gates = unpack(args[5], "gates"),
                slots = unpack(args[6], "slots");
@@ -627,6 +636,7 @@ FOX_PY(py_paged_update) {
 // (q, k_pages, v_pages, gate_pages, block_table, lengths, sm_scale or None, return_log_normalizer) -> out or (out, L)
 FOX_PY(py_paged_attention) {
   HANDLE_TH_ERRORS
+  not_traced("paged_forgetting_attention");
   const Tensor q_in = unpack(args[0], "q"), kp = unpack(args[1], "k_pages"), vp = unpack(args[2], "v_pages"),
                gp = unpack(args[3], "gate_pages"), table = unpack(args[4], "block_table"), lengths = unpack(args[5], "lengths");
   const double given = args[6] == Py_None ? 0. : number(args[6]);

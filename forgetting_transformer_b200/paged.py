@@ -11,6 +11,8 @@ read and change them: nothing here waits for the GPU, and a step can be captured
         cache.update(layer, k, v, log_fgate, t.slots)
         o = cache.attend(layer, q)                            # (max_requests, heads, head_dim): one query per request
     cache.release(finished)                                   # (max_requests,) bool
+
+All of it works in place, so that torch.jit.trace refuses it (a trace would keep the results and drop the writes).
 """
 from __future__ import annotations
 

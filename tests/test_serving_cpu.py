@@ -201,3 +201,22 @@ def test_one_request_out_of_many_columns():
         fox.page_tables(state[:, 0], state[:, 1], i(1, 3), i(5), state[:, 2], 16, 4)
     with pytest.raises(AssertionError, match="contiguous"):
         fox.page_tables(i(2, 3)[:, 0], i(2), i(2, 3), i(5), i(1), 16, 4)
+
+
+def paged_calls():
+    """Each paged operator on valid arguments, as a function of those of them that may carry values: (name, function, inputs)."""
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    k, v, g = pages()
+    q, rows, gates = bf(3, 2, 64), bf(4, 2, 64), torch.zeros(4, 2)
+    return [("page_tables", lambda n: fox.page_tables(i(2), n, i(2, 3), i(5), i(1), 16, 4), (i(2),)),
+            ("release_pages", lambda n: fox.release_pages(i(2), n, i(2, 3), i(5), i(1), 16), (i(2),)),
+            ("paged_update", lambda *a: fox.paged_update(*a, i(4)), (k, v, g, rows, rows.clone(), gates)),
+            ("paged_forgetting_attention", lambda *a: fox.paged_forgetting_attention(*a, i(3, 4), i(3)), (q, k, v, g))]
+
+
+@pytest.mark.parametrize("which", range(4))
+def test_paged_operators_are_not_traced(which):
+    """A trace would keep the first call's results for every input, and none of the writes."""
+    name, f, args = paged_calls()[which]
+    with torch.no_grad(), pytest.raises(_lib.FoxError, match=name + " cannot be traced"):
+        torch.jit.trace(f, args, check_trace=False)
