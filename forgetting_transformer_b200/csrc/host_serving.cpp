@@ -343,6 +343,11 @@ int64_t table_ld(const Tensor& t) { return t.size(0) == 1 ? t.size(1) : t.stride
 void not_traced(const char* what) {
   if (tracing()) raise_fox(std::string(what) + " cannot be traced: its results would be constants of the trace, and its writes lost");
 }
+// (a result would come back without its tangent, and what is written without it too)
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (has_tangent(*t)) raise_fox(std::string(what) + " has no forward-mode derivatives: its inputs may carry no tangents");
+}
 
 struct Pool {   // the pages of one layer
   Tensor k, v, gates;
@@ -610,6 +615,7 @@ FOX_PY(py_paged_update) {
     if (at::GradMode::is_enabled() && (k_in.requires_grad() || v_in.requires_grad() || gates.requires_grad() || kp.requires_grad() ||
                                        vp.requires_grad() || gp.requires_grad()))
       raise_fox("paged_update has no gradients: call it under torch.no_grad()");
+    no_tangents("paged_update", {&k_in, &v_in, &gates, &kp, &vp, &gp});
     need_cuda(kp, "paged_update");
     same_device("paged_update", kp, {&vp, &gp, &k_in, &v_in, &gates, &slots});
     const c10::cuda::CUDAGuard guard(kp.device());
@@ -655,6 +661,7 @@ FOX_PY(py_paged_attention) {
     check_that(R == 0 || table.size(1) == 0 || table_ld(table) >= table.size(1), "rows of block_table must not overlap");
     if (at::GradMode::is_enabled() && (q_in.requires_grad() || kp.requires_grad() || vp.requires_grad() || gp.requires_grad()))
       raise_fox("paged_forgetting_attention has no gradients: call it under torch.no_grad()");
+    no_tangents("paged_forgetting_attention", {&q_in, &kp, &vp, &gp});
     need_cuda(q_in, "paged_forgetting_attention");
     same_device("paged_forgetting_attention", q_in, {&kp, &vp, &gp, &table, &lengths});
     const c10::cuda::CUDAGuard guard(q_in.device());

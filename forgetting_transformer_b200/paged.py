@@ -76,7 +76,7 @@ def paged_update(k_pages: torch.Tensor, v_pages: torch.Tensor, gate_pages: torch
     k_pages, v_pages (pages, Hk, page_size, D) in fp16 / bf16, rows contiguous and 16-byte aligned; gate_pages (pages, H,
     page_size) fp32; slots (T,) int32 / int64.  A slot outside the pool (-1) leaves its token out; of tokens with the same slot
     any one's values may stay, piece by piece.  ``gate_is_logit``: the gates are logits (fp16 / bf16 / fp32) and their log
-    sigmoid is written.  No gradients."""
+    sigmoid is written.  No gradients and no tangents."""
     (_host or _load_host()).paged_update(k_pages, v_pages, gate_pages, k, v, log_fgate, slots, gate_is_logit)
 
 
@@ -89,7 +89,8 @@ def paged_forgetting_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: 
     Pages as for ``paged_update`` (gates 16-byte aligned too); H is a multiple of the pages' heads Hk, and H / Hk query heads
     share a key head, each with gates of its own.  A request of length 0 gets zeros.  Entries of ``block_table`` behind a request's
     length are not looked at; one in front of it that is outside the pool leaves its keys out.  ``return_log_normalizer``: also
-    the (R, H) log-sum-exp of the logits (-inf without keys).  No gradients."""
+    the (R, H) log-sum-exp of the logits (-inf without keys).  No gradients and no
+    tangents."""
     return (_host or _load_host()).paged_attention(q, k_pages, v_pages, gate_pages, block_table, lengths, sm_scale,
                                                    return_log_normalizer)
 

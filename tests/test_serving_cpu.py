@@ -5,6 +5,7 @@ import pickle
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import forgetting_transformer_b200 as fox
 from forgetting_transformer_b200 import _lib
@@ -220,3 +221,13 @@ def test_paged_operators_are_not_traced(which):
     name, f, args = paged_calls()[which]
     with torch.no_grad(), pytest.raises(_lib.FoxError, match=name + " cannot be traced"):
         torch.jit.trace(f, args, check_trace=False)
+
+
+@pytest.mark.parametrize("which,at", [(2, i) for i in range(6)] + [(3, i) for i in range(4)])
+def test_paged_operators_have_no_forward_mode(which, at):
+    """A dual tensor, of values or of pages, raises: nothing comes back, or is written, without its tangent."""
+    name, f, args = paged_calls()[which]
+    with fwAD.dual_level(), torch.no_grad():
+        args = [fwAD.make_dual(t, torch.ones_like(t)) if i == at else t for i, t in enumerate(args)]
+        with pytest.raises(_lib.FoxError, match=name + " has no forward-mode"):
+            f(*args)
