@@ -95,6 +95,7 @@ void check_rotation(Rotation& r, const Rows& s, const Tensor& x, const char* wha
   check_that(r.inv_freq.dim() == 1 && r.inv_freq.scalar_type() == at::kFloat, "inv_freq must be a vector in torch.float32");
   if (at::GradMode::is_enabled() && r.inv_freq.requires_grad())
     raise_fox(std::string(what) + " has no gradient for inv_freq: detach it, or call it under torch.no_grad()");
+  if (has_tangent(r.inv_freq)) raise_fox(std::string(what) + " has no forward-mode derivative for inv_freq: it may carry no tangent");
   r.half = r.inv_freq.numel();
   check_that(r.half >= 1 && 2 * r.half <= s.D, "inv_freq must have between 1 and head dim / 2 elements");
   if (r.positions.defined()) {

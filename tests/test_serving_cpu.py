@@ -231,3 +231,12 @@ def test_paged_operators_have_no_forward_mode(which, at):
         args = [fwAD.make_dual(t, torch.ones_like(t)) if i == at else t for i, t in enumerate(args)]
         with pytest.raises(_lib.FoxError, match=name + " has no forward-mode"):
             f(*args)
+
+
+def test_frequencies_have_no_forward_mode():
+    with fwAD.dual_level(), torch.no_grad():
+        f = fwAD.make_dual(F32, torch.ones_like(F32))
+        with pytest.raises(_lib.FoxError, match="no forward-mode derivative for inv_freq"):
+            fox.rotary_embedding(bf(1, 4, 2, 64), f)
+        with pytest.raises(_lib.FoxError, match="no forward-mode derivative for inv_freq"):
+            fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 2, 64), torch.ones(64), torch.ones(64), f)
