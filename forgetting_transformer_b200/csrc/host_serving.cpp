@@ -49,6 +49,14 @@ void written(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (!t->is_inference()) torch::autograd::impl::bump_version(*t);
 }
+// An argument whose memory a kernel will be given.  (A subclass that only wraps other tensors has none: its address is its offset.)
+const Tensor& held(PyObject* o, const char* what) {
+  const Tensor& t = unpack(o, what);
+  if (t.unsafeGetTensorImpl()->is_python_dispatch() && t.numel() && !t.storage().data())
+    raise_fox(std::string(what) + " is of a tensor subclass that holds no memory of its own");
+  return t;
+}
+Tensor held_opt(PyObject* o, const char* what) { return o == Py_None ? Tensor() : held(o, what); }
 double number(PyObject* o) {
   const double x = PyFloat_AsDouble(o);
   if (PyErr_Occurred()) throw python_error();
@@ -312,9 +320,9 @@ NormSaved norm_inputs(const Tensor& q, const Tensor& k, const Tensor& wq, const 
 
 Rotation parse_rotation(PyObject* inv_freq, PyObject* positions, PyObject* head_first, PyObject* interleaved, PyObject* scale) {
   Rotation r;
-  r.inv_freq = unpack(inv_freq, "inv_freq");
+  r.inv_freq = held(inv_freq, "inv_freq");
   if (positions != Py_None) {
-    if (THPVariable_Check(positions)) r.positions = THPVariable_Unpack(positions);
+    if (THPVariable_Check(positions)) r.positions = held(positions, "positions");
     else r.first = integer(positions, "positions (where they are not a tensor)");
   }
   r.head_first = PyObject_IsTrue(head_first) == 1;
@@ -393,7 +401,7 @@ FOX_PY(py_rotary) {
   if (tracing()) Py_RETURN_NONE;
   for (int i = 0; i < 3; ++i)
     if (THPVariable_Check(args[i]) && !plain_tensor(args[i])) Py_RETURN_NONE;
-  const Tensor x = unpack(args[0], "x");
+  const Tensor x = held(args[0], "x");
   Rotation r = parse_rotation(args[1], args[2], args[3], args[4], args[5]);
   if (has_tangent(x)) Py_RETURN_NONE;
   Tensor y;
@@ -411,7 +419,7 @@ FOX_PY(py_rotary) {
 // (x, inv_freq, positions, head_first, interleaved, scale, inverse) -> y, without an autograd node
 FOX_PY(py_rotary_apply) {
   HANDLE_TH_ERRORS
-  const Tensor x = unpack(args[0], "x");
+  const Tensor x = held(args[0], "x");
   Rotation r = parse_rotation(args[1], args[2], args[3], args[4], args[5]);
   const bool inverse = PyObject_IsTrue(args[6]) == 1;
   Tensor y;
@@ -431,7 +439,7 @@ FOX_PY(py_qk_norm_rotary) {
   if (tracing()) Py_RETURN_NONE;
   for (int i = 0; i < 6; ++i)
     if (THPVariable_Check(args[i]) && !plain_tensor(args[i])) Py_RETURN_NONE;
-  const Tensor q = unpack(args[0], "q"), k = unpack(args[1], "k"), wq = unpack(args[2], "q_weight"), wk = unpack(args[3], "k_weight");
+  const Tensor q = held(args[0], "q"), k = held(args[1], "k"), wq = held(args[2], "q_weight"), wk = held(args[3], "k_weight");
   Rotation r = parse_rotation(args[4], args[5], args[7], args[8], args[9]);
   r.eps = number(args[6]);
   for (const Tensor* t : {&q, &k, &wq, &wk})
@@ -464,7 +472,7 @@ FOX_PY(py_qk_norm_rotary) {
 // the ten arguments -> (q, k), without an autograd node
 FOX_PY(py_qk_norm_rotary_forward) {
   HANDLE_TH_ERRORS
-  const Tensor q = unpack(args[0], "q"), k = unpack(args[1], "k"), wq = unpack(args[2], "q_weight"), wk = unpack(args[3], "k_weight");
+  const Tensor q = held(args[0], "q"), k = held(args[1], "k"), wq = held(args[2], "q_weight"), wk = held(args[3], "k_weight");
   Rotation r = parse_rotation(args[4], args[5], args[7], args[8], args[9]);
   r.eps = number(args[6]);
   std::array<Tensor, 2> out;
@@ -479,10 +487,10 @@ FOX_PY(py_qk_norm_rotary_forward) {
 // (the ten arguments, gradients of both results or None) -> (dq, dk, dq_weight, dk_weight)
 FOX_PY(py_qk_norm_rotary_backward) {
   HANDLE_TH_ERRORS
-  const Tensor q = unpack(args[0], "q"), k = unpack(args[1], "k"), wq = unpack(args[2], "q_weight"), wk = unpack(args[3], "k_weight");
+  const Tensor q = held(args[0], "q"), k = held(args[1], "k"), wq = held(args[2], "q_weight"), wk = held(args[3], "k_weight");
   Rotation r = parse_rotation(args[4], args[5], args[7], args[8], args[9]);
   r.eps = number(args[6]);
-  const Tensor gq = unpack_opt(args[10], "dq"), gk = unpack_opt(args[11], "dk");
+  const Tensor gq = held_opt(args[10], "dq"), gk = held_opt(args[11], "dk");
   std::array<Tensor, 4> g;
   {
     pybind11::gil_scoped_release no_gil;
@@ -499,8 +507,8 @@ FOX_PY(py_qk_norm_rotary_backward) {
 FOX_PY(py_page_tables) {
   HANDLE_TH_ERRORS
   not_traced("page_tables");
-  const Tensor lengths = unpack(args[0], "lengths"), fresh = unpack(args[1], "new_tokens"), table = unpack(args[2], "block_table"),
-               pages = unpack(args[3], "free_pages"), num_free = unpack(args[4], "num_free");
+  const Tensor lengths = held(args[0], "lengths"), fresh = held(args[1], "new_tokens"), table = held(args[2], "block_table"),
+               pages = held(args[3], "free_pages"), num_free = held(args[4], "num_free");
   const int64_t page = integer(args[5], "page_size"), T = integer(args[6], "max_tokens");
   const bool inplace = PyObject_IsTrue(args[7]) == 1;
   std::array<Tensor, 7> out;
@@ -555,8 +563,8 @@ FOX_PY(py_page_tables) {
 FOX_PY(py_release_pages) {
   HANDLE_TH_ERRORS
   not_traced("release_pages");
-  const Tensor lengths = unpack(args[0], "lengths"), keep = unpack(args[1], "keep"), table = unpack(args[2], "block_table"),
-               pages = unpack(args[3], "free_pages"), num_free = unpack(args[4], "num_free");
+  const Tensor lengths = held(args[0], "lengths"), keep = held(args[1], "keep"), table = held(args[2], "block_table"),
+               pages = held(args[3], "free_pages"), num_free = held(args[4], "num_free");
   const int64_t page = integer(args[5], "page_size");
   {
     pybind11::gil_scoped_release no_gil;
@@ -592,9 +600,9 @@ FOX_PY(py_release_pages) {
 FOX_PY(py_paged_update) {
   HANDLE_TH_ERRORS
   not_traced("paged_update");
-  const Tensor kp = unpack(args[0], "k_pages"), vp = unpack(args[1], "v_pages"), gp = unpack(args[2], "gate_pages");
-  const Tensor k_in = unpack(args[3], "k"), v_in = unpack(args[4], "v"), gates = unpack(args[5], "gates"),
-               slots = unpack(args[6], "slots");
+  const Tensor kp = held(args[0], "k_pages"), vp = held(args[1], "v_pages"), gp = held(args[2], "gate_pages");
+  const Tensor k_in = held(args[3], "k"), v_in = held(args[4], "v"), gates = held(args[5], "gates"),
+               slots = held(args[6], "slots");
   const bool logit = PyObject_IsTrue(args[7]) == 1;
   {
     pybind11::gil_scoped_release no_gil;
@@ -644,8 +652,8 @@ FOX_PY(py_paged_update) {
 FOX_PY(py_paged_attention) {
   HANDLE_TH_ERRORS
   not_traced("paged_forgetting_attention");
-  const Tensor q_in = unpack(args[0], "q"), kp = unpack(args[1], "k_pages"), vp = unpack(args[2], "v_pages"),
-               gp = unpack(args[3], "gate_pages"), table = unpack(args[4], "block_table"), lengths = unpack(args[5], "lengths");
+  const Tensor q_in = held(args[0], "q"), kp = held(args[1], "k_pages"), vp = held(args[2], "v_pages"),
+               gp = held(args[3], "gate_pages"), table = held(args[4], "block_table"), lengths = held(args[5], "lengths");
   const double given = args[6] == Py_None ? 0. : number(args[6]);
   const bool want_L = PyObject_IsTrue(args[7]) == 1;
   Tensor o, L;

@@ -240,3 +240,37 @@ def test_frequencies_have_no_forward_mode():
             fox.rotary_embedding(bf(1, 4, 2, 64), f)
         with pytest.raises(_lib.FoxError, match="no forward-mode derivative for inv_freq"):
             fox.qk_norm_rotary(bf(1, 4, 2, 64), bf(1, 4, 2, 64), torch.ones(64), torch.ones(64), f)
+
+
+class Wrapper(torch.Tensor):
+    """A subclass that holds no memory: its data pointer is the offset it was given."""
+
+    @staticmethod
+    def __new__(cls, t):
+        return torch.Tensor._make_wrapper_subclass(cls, t.shape, strides=t.stride(), storage_offset=64, dtype=t.dtype, device=t.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise RuntimeError(f"{func} was not meant to run")
+
+
+@pytest.mark.parametrize("which,at", [(0, 0), (1, 0)] + [(2, i) for i in range(6)] + [(3, i) for i in range(4)])
+def test_wrapped_tensors_never_reach_a_paged_kernel(which, at):
+    _, f, args = paged_calls()[which]
+    assert Wrapper(args[at]).data_ptr() == 64 * args[at].element_size()
+    with torch.no_grad(), pytest.raises(_lib.FoxError, match="holds no memory"):
+        f(*(Wrapper(t) if i == at else t for i, t in enumerate(args)))
+
+
+@pytest.mark.parametrize("at", range(6))
+def test_wrapped_tensors_never_reach_a_rotary_kernel(at):
+    """Nor through the autograd functions, which take what the native nodes leave to them."""
+    w = torch.ones(64)
+    args = [bf(1, 4, 2, 64), bf(1, 4, 2, 64), w, w.clone(), F32, torch.zeros(4, dtype=torch.int32)]
+    args[at] = Wrapper(args[at])
+    calls = [lambda: fox.qk_norm_rotary(*args)]
+    if at in (0, 4, 5):
+        calls.append(lambda: fox.rotary_embedding(args[0], args[4], args[5]))
+    for call in calls:
+        with pytest.raises(_lib.FoxError, match="holds no memory"):
+            call()
