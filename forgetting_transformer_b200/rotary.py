@@ -98,6 +98,12 @@ class _NormRotate(torch.autograd.Function):
         return (*_lib.host().qk_norm_rotary_backward(*tensors, at, *ctx.rest, dq, dk), None, None, None, None, None, None)
 
 
+def _no_frequency_gradient(what: str, inv_freq: torch.Tensor) -> None:
+    """(The native nodes look for themselves; inside an autograd function's forward gradients are off.)"""
+    if torch.is_grad_enabled() and inv_freq.requires_grad:
+        raise _lib.FoxError(f"{what} has no gradient for inv_freq: detach it, or call it under torch.no_grad()")
+
+
 def rotary_embedding(x: torch.Tensor, inv_freq: torch.Tensor, positions: Positions = None, *, head_first: bool = False,
                      interleaved: bool = False, scale: float = 1.0) -> torch.Tensor:
     """``x`` with the first ``2 * inv_freq.numel()`` channels of every head turned by ``position * inv_freq`` and multiplied
@@ -112,7 +118,10 @@ def rotary_embedding(x: torch.Tensor, inv_freq: torch.Tensor, positions: Positio
     Differentiable w.r.t. x, any number of times."""
     pos = 0 if positions is None else positions
     out = (_host or _load_host()).rotary(x, inv_freq, pos, head_first, interleaved, scale)
-    return _Rotate.apply(x, inv_freq, pos, head_first, interleaved, scale) if out is None else out
+    if out is None:
+        _no_frequency_gradient("rotary_embedding", inv_freq)
+        out = _Rotate.apply(x, inv_freq, pos, head_first, interleaved, scale)
+    return out
 
 
 def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, inv_freq: torch.Tensor,
@@ -124,8 +133,10 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
     alike, k_weight likewise, fp16 / bf16 / fp32.  Returns (q, k); differentiable, once, w.r.t. q, k and both weights."""
     pos = 0 if positions is None else positions
     out = (_host or _load_host()).qk_norm_rotary(q, k, q_weight, k_weight, inv_freq, pos, eps, head_first, interleaved, scale)
-    return (_NormRotate.apply(q, k, q_weight, k_weight, inv_freq, pos, eps, head_first, interleaved, scale)
-            if out is None else out)
+    if out is None:
+        _no_frequency_gradient("qk_norm_rotary", inv_freq)
+        out = _NormRotate.apply(q, k, q_weight, k_weight, inv_freq, pos, eps, head_first, interleaved, scale)
+    return out
 
 
 class RotaryEmbedding(nn.Module):

@@ -274,3 +274,11 @@ def test_wrapped_tensors_never_reach_a_rotary_kernel(at):
     for call in calls:
         with pytest.raises(_lib.FoxError, match="holds no memory"):
             call()
+
+
+def test_frequencies_have_no_gradient_where_the_call_is_traced():
+    f, w = F32.clone().requires_grad_(), torch.ones(64)
+    with pytest.raises(_lib.FoxError, match="rotary_embedding has no gradient for inv_freq"):
+        torch.jit.trace(lambda x: fox.rotary_embedding(x, f), (bf(1, 4, 2, 64),), check_trace=False)
+    with pytest.raises(_lib.FoxError, match="qk_norm_rotary has no gradient for inv_freq"):
+        torch.jit.trace(lambda x: fox.qk_norm_rotary(x, x, w, w, f), (bf(1, 4, 2, 64),), check_trace=False)
