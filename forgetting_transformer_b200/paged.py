@@ -148,9 +148,16 @@ class PagedFgateCache:
         self.crop(torch.where(requests, 0, self.lengths))
 
     def history(self, layer_idx: int, request: int, length: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-        """The first ``length`` tokens of a request as ``forgetting_attention`` takes them, head-first: k, v (1, Hk, length, D) and
-        log gates (1, H, length); copies, for a prompt that comes in several chunks."""
-        pages = self.block_table[request, :-(-length // self.page_size)].long()
-        k, v, g = [t[layer_idx][pages].transpose(0, 1).flatten(1, 2)[None, :, :length]
-                   for t in (self.k_pages, self.v_pages, self.gate_pages)]
-        return k, v, g
+        """The first ``length`` tokens of a request, head-first: k, v (1, Hk, length, D) and log gates (1, H, length); copies, for a
+        prompt that comes in several chunks.  Tokens behind the request's end are zeros, not what their places last held."""
+        P, most = self.k_pages.shape[1], self.block_table.shape[1] * self.page_size
+        if not 0 <= length <= most:
+            raise ValueError(f"a request holds 0 to {most} tokens, but got a length of {length}")
+        at = torch.arange(length, device=self.lengths.device)
+        pages, rows = self.block_table[request].long()[at // self.page_size], at % self.page_size
+        absent = (at >= self.lengths[request]) | (pages < 0) | (pages >= P)
+        pages = pages.clamp(0, P - 1)
+        k, v, g = [t[layer_idx].transpose(0, 1)[:, pages, rows][None] for t in (self.k_pages, self.v_pages, self.gate_pages)]
+        for t in (k, v):
+            t.masked_fill_(absent[:, None], 0)
+        return k, v, g.masked_fill_(absent, 0)

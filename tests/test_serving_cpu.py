@@ -282,3 +282,28 @@ def test_frequencies_have_no_gradient_where_the_call_is_traced():
         torch.jit.trace(lambda x: fox.rotary_embedding(x, f), (bf(1, 4, 2, 64),), check_trace=False)
     with pytest.raises(_lib.FoxError, match="qk_norm_rotary has no gradient for inv_freq"):
         torch.jit.trace(lambda x: fox.qk_norm_rotary(x, x, w, w, f), (bf(1, 4, 2, 64),), check_trace=False)
+
+
+def test_history_ends_with_the_request():
+    """What is asked for behind a request's end, in its last page or in pages that it does not own, is zero: not the rows of
+    another request, nor what the memory held before."""
+    c = fox.PagedFgateCache(num_layers=2, num_pages=4, page_size=16, num_heads=4, num_kv_heads=2, head_dim=16, max_requests=3,
+                            max_length=64, device="cpu")
+    for n, t in enumerate((c.k_pages, c.v_pages, c.gate_pages)):
+        t.copy_((torch.arange(t.numel()).view(t.shape) % 997 + 1 + n).to(t.dtype))
+    c.block_table[0, :2] = torch.tensor([2, 0], dtype=torch.int32)
+    c.block_table[1, :1] = 3
+    c.lengths.copy_(torch.tensor([21, 16, 0]))
+    for request, ids, have in ((0, [2, 0], 21), (1, [3], 16), (2, [], 0)):
+        for length in (0, have // 2, have, have + 1, 48, 64):
+            got = c.history(1, request, length)
+            n = min(have, length)
+            for t, pool in zip(got, (c.k_pages, c.v_pages, c.gate_pages)):
+                want = torch.cat([pool[1, p] for p in ids], 1)[:, :n] if ids else pool[1, 0, :, :0]
+                assert t.shape == (1, pool.shape[2], length, *pool.shape[4:]) and t.is_contiguous()
+                assert torch.equal(t[0, :, :n], want) and not t[0, :, n:].any()
+    c.block_table[0, 1] = 2 ** 30       # (an entry outside the pool: its keys take no part in the attention either)
+    assert not c.history(0, 0, 21)[0][0, :, 16:].any()
+    for length in (-1, 65):
+        with pytest.raises(ValueError, match="0 to 64 tokens"):
+            c.history(0, 0, length)
