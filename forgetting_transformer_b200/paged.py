@@ -149,7 +149,8 @@ class PagedFgateCache:
 
     def history(self, layer_idx: int, request: int, length: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """The first ``length`` tokens of a request, head-first: k, v (1, Hk, length, D) and log gates (1, H, length); copies, for a
-        prompt that comes in several chunks.  Tokens behind the request's end are zeros, not what their places last held."""
+        prompt that comes in several chunks.  ``forgetting_attention`` takes them as they are where Hk = H, else k and v with their
+        heads repeated (``repeat_interleave(H // Hk, 1)``).  Tokens behind the request's end are zeros, not what their places last held."""
         P, most = self.k_pages.shape[1], self.block_table.shape[1] * self.page_size
         if not 0 <= length <= most:
             raise ValueError(f"a request holds 0 to {most} tokens, but got a length of {length}")
