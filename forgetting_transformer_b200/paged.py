@@ -56,6 +56,9 @@ def page_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: to
       taken first.  All int32 on one device.
     - Requests are served in their order.  One whose tokens find no room (in its table row, among ``max_tokens``, or pages) is
       granted none and keeps its length; its tokens have slot -1, which ``paged_update`` leaves out.
+    - Nobody overtakes: after a request that the free pages were too few for, those behind it get no page in this call either (new
+      tokens that fit into their last page are granted), and tokens count towards ``max_tokens`` whether granted or not.  Set
+      ``new_tokens`` to 0 for a request that is to wait.
     - ``inplace``: lengths and num_free are changed instead of returned anew.
     - page_size: a power of two from 16 to 65536."""
     return PageTables._make((_host or _load_host()).page_tables(lengths, new_tokens, block_table, free_pages, num_free, page_size,

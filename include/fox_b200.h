@@ -487,7 +487,8 @@ int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64_t B, int64
  *
  * Pages for new_tokens[r] more tokens of every request, in order: lengths_out = lengths + what was granted, the table's new
  * entries, num_free_out, starts (R + 1) = the packed batch's first token of every request, granted (R) = new_tokens, or 0 for a
- * request whose tokens find no room (its table row of `width` entries, max_tokens, the free pages), and for each of the packed
+ * request whose tokens find no room (its table row of `width` entries, max_tokens, the free pages; after one that the free pages were
+ * too few for, those behind it get no page either, and tokens that are not granted count towards max_tokens all the same), and for each of the packed
  * batch's max_tokens places its request (-1: none), position (0) and slot (-1: none, or not granted).  lengths_out and
  * num_free_out may be lengths and num_free.  workspace: R + 1. */
 int fox_page_tables(int device, void* stream, int64_t R, int64_t width, int64_t page, int64_t max_tokens, const int32_t* lengths,
