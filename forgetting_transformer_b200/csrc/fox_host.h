@@ -143,13 +143,16 @@ inline int cached_tmap_4d(CUtensorMap* out, const Tensor4& t, int elem_bytes, bo
 }
 
 // Launches a kernel whose CTAs may take their SMs and set up their barriers as soon as the last CTA of the kernel in front has ended,
-// before its results are written back; the kernel calls wait_for_kernel_in_front() before it reads or writes memory (its loads must
-// not be __restrict__ or .nc ones, which may be done in front of the wait).  A launch behind another by stream order alone costs 1.5-2 us from
-// the end of the first to the first load of the second; a pass of the attention is 5 to 7 kernels.  Forward and backward
-// together, back to back, stream order -> this: B1 H2 T128 D64 30.9 -> 22.4 us, B4 H12 T512 D64 51.2 -> 41.0, B2 H16 T2048 D128
-// 215 -> 203, B1 H24 T4096 D64 313 -> 301; from some 500 us a pass on within the noise.  None of the kernels lets the next begin
-// earlier than that: a forward begun when its prefix sums had begun had its CTAs packed around theirs, on fewer SMs (B2 H7
-// M700 N1500 D128 36.9 us by stream order, 39.5 so, 34.7 as here; B1 H4 T9000 D128 144, 157, 141).
+// before its results are written back, or has let it begin (griddepcontrol.launch_dependents: the scan of large page tables, both kernels
+// of the paged attention and those of a generation step do that near their start, so that the kernel in front may still be running all
+// through).  So the kernel calls wait_for_kernel_in_front() before it reads or writes memory that one in front writes or reads, before it
+// lets another begin, and before it ends, whether it has work or not: what comes behind it by stream order relies on its end alone.  (Its
+// loads must not be __restrict__ or .nc ones, which may be done in front of the wait.)  A launch behind another by stream order alone
+// costs 1.5-2 us from the end of the first to the first load of the second; a pass of the attention is 5 to 7 kernels.  Forward and
+// backward together, back to back, stream order -> this: B1 H2 T128 D64 30.9 -> 22.4 us, B4 H12 T512 D64 51.2 -> 41.0, B2 H16 T2048 D128
+// 215 -> 203, B1 H24 T4096 D64 313 -> 301; from some 500 us a pass on within the noise.  None of the training kernels lets the next begin
+// before its own end: a forward begun when its prefix sums had begun had its CTAs packed around theirs, on fewer SMs (B2 H7 M700 N1500
+// D128 36.9 us by stream order, 39.5 so, 34.7 as here; B1 H4 T9000 D128 144, 157, 141).
 // The kernels of a block's training pass between the products go the same way (forward and backward, all on the device: B4 T512 of 768
 // channels 282 -> 265 us, B4 T1024 of 1024 593 -> 575, B1 T16384 of 1536 within the noise), but for its row norms: without
 // __restrict__ their loads are issued later (backward, 16384 x 1536: 46 -> 86 us).
