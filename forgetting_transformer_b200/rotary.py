@@ -142,7 +142,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_w
 class RotaryEmbedding(nn.Module):
     """Rotary positions of a layer: ``rotary_frequencies``' arguments, kept with the layout of the pairs.  ``forward`` rotates
     q and k; ``norm`` norms them first.  The frequencies stay in fp32 whatever type the module is moved to; they come from the
-    arguments, so that a module built on the meta device has them too, and what is pickled holds no device's copy."""
+    arguments, so that a module built on the meta device has them too, and what is pickled holds no device's copy.  They are copied
+    to a device at the first call there, which may not be one that is captured in a CUDA graph."""
 
     def __init__(self, dim: int, base: float = 10000.0, interleaved: bool = False, **scaling):
         super().__init__()
@@ -157,6 +158,9 @@ class RotaryEmbedding(nn.Module):
     def inv_freq(self, device) -> torch.Tensor:
         got = self._on_device.get(device)
         if got is None:
+            if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+                raise _lib.FoxError("the frequencies come to a device at the first call there, which cannot be captured in a graph: "
+                                    "call the module, or its inv_freq(device), once before")
             with torch.inference_mode(False):   # (the copy serves training too)
                 got = self._freq.to(device)
             if type(got) is torch.Tensor:       # (a tracer's stand-in is not kept)

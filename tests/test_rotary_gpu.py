@@ -428,3 +428,27 @@ def test_many_tokens(T, H, D):
     for got, src, slack in ((y, x.double(), 2 ** -20), (q, n, 2 ** -19), (k, n, 2 ** -19)):
         ref = turn64(src, a, False)
         assert ((got.double() - ref).abs() <= 2 ** -8 * ref.abs() + slack * reach(src, D // 2, False)).all()
+
+
+def test_module_in_a_capture():
+    """A module whose frequencies are not yet on the device refuses to be captured, without harm to the capture; one that has been
+    called, or asked for them, is replayed on new values."""
+    m = fox.RotaryEmbedding(64)
+    q, k = [data(i, 1, 9, 2, 64, dtype=torch.bfloat16) for i in range(2)]
+    stays = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        with pytest.raises(fox.FoxError, match="once before"):
+            m(q, k, 5)
+        stays.add_(1)
+    g.replay()
+    assert stays.tolist() == [1.0] * 4
+    m.inv_freq(q.device)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = m(q, k, 5)
+    q.copy_(data(3, 1, 9, 2, 64, dtype=torch.bfloat16))
+    g.replay()
+    for a, b in zip(got, m(q, k, 5)):
+        assert torch.equal(a, b)

@@ -307,3 +307,13 @@ def test_history_ends_with_the_request():
     for length in (-1, 65):
         with pytest.raises(ValueError, match="0 to 64 tokens"):
             c.history(0, 0, length)
+
+
+def test_module_refuses_its_first_call_in_a_capture(monkeypatch):
+    """The copy from the host would end the capture; the refusal comes before it, and a device that has its copy needs none."""
+    m, gpu = fox.RotaryEmbedding(64), torch.device("cuda", 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(_lib.FoxError, match="once before"):
+        m.inv_freq(gpu)
+    m._on_device[gpu] = F32
+    assert m.inv_freq(gpu) is F32 and m.inv_freq(torch.device("cpu")).shape == (32,)
