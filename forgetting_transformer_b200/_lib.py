@@ -124,6 +124,7 @@ _SIGNATURES = {
     "fox_qk_norm_rotary_fwd": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, _T4P, _T4P, _F,
                         c_int, c_int64, _F, c_int, c_int64, c_float, _F, c_int64, c_int, c_float, _F, c_int, c_int64,
                         c_int64, c_int64, _T4P, _T4P]),
+    "fox_rotary_range": (c_int64, [c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
     "fox_qk_norm_rotary_partials": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64]),
     "fox_qk_norm_rotary_bwd": (c_int, [c_int, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, _T4P, _T4P, _F,
                         c_int, c_int64, _F, c_int, c_int64, c_float, _F, c_int64, c_int, c_float, _F, c_int, c_int64,

@@ -479,6 +479,10 @@ int fox_qk_norm_rotary_bwd(int device, void* stream, int dtype, int64_t B, int64
                            int64_t first, const fox_tensor4* dq_out, const fox_tensor4* dk_out, const fox_tensor4* dq,
                            const fox_tensor4* dk, float* dw_partial, void* dwq, void* dwk);
 
+/* Tokens that a CTA of these launches goes through, which it does in tiles of 32 (pairs in halves that are no multiple of 4: of 16),
+ * each of one sequence's tokens.  kind: 0 fox_rotary, 1 fox_qk_norm_rotary_fwd, 2 fox_qk_norm_rotary_bwd; heads: H + Hk. */
+int64_t fox_rotary_range(int kind, int64_t B, int64_t T, int64_t heads, int64_t D, int64_t half, int interleaved);
+
 /* ---------------------------------------------------------------- paged generation cache
  * The counterpart of upstream's growing cache (fgate_cache.py:77-116) for requests of different lengths.  A pool of n_pages
  * pages of `page` tokens (a power of two, 16 to 65536); token t of request r is row t % page of page

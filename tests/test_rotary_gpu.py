@@ -452,3 +452,86 @@ def test_module_in_a_capture():
     g.replay()
     for a, b in zip(got, m(q, k, 5)):
         assert torch.equal(a, b)
+
+
+def big(seed, *shape, dtype):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dtype)
+
+
+def several_tiles(kind, B, T, heads, D, rot, interleaved):
+    """Whether a CTA's range of tokens is longer than the tile whose angles it holds, so that it comes to a second one; and, with
+    sequences that are no multiple of the range, crosses from one into the next."""
+    from forgetting_transformer_b200 import _lib
+    per = _lib.load().fox_rotary_range(kind, B, T, heads, D, rot // 2, interleaved)
+    return per > (16 if not interleaved and rot // 2 % 4 else 32) and T % per
+
+
+@pytest.mark.parametrize("T,H,D,rot,interleaved,head_first,dtype", [
+    (25603, 16, 128, 128, False, False, torch.bfloat16), (25603, 32, 64, 64, True, False, torch.float16),
+    (25603, 32, 64, 32, False, True, torch.float16), (25603, 128, 16, 12, True, False, torch.bfloat16),
+    (25603, 64, 32, 32, False, False, torch.bfloat16), (4001, 16, 128, 44, False, False, torch.bfloat16),
+    (4001, 16, 128, 42, False, True, torch.float16), (8001, 16, 64, 22, False, False, torch.float16),
+    (8001, 64, 16, 12, False, False, torch.bfloat16)])
+def test_rotary_of_ranges_in_several_tiles(T, H, D, rot, interleaved, head_first, dtype):
+    """Ranges of more tokens than a tile, across sequences with positions of their own; the gradient is the same kernel."""
+    B = 3
+    assert several_tiles(0, B, T, H, D, rot, interleaved)
+    inv_freq, _ = fox.rotary_frequencies(rot, device="cuda")
+    pos = torch.randint(0, 50000, (B, T), generator=torch.Generator().manual_seed(T)).int().cuda()
+    lay = (lambda t: t.transpose(1, 2)) if head_first else (lambda t: t)
+    x, dy = [lay(big(T + i, *((B, H, T, D) if head_first else (B, T, H, D)), dtype=dtype)) for i in range(2)]
+    xin = lay(x).detach().requires_grad_()
+    y = fox.rotary_embedding(xin, inv_freq, pos, head_first=head_first, interleaved=interleaved)
+    (dx,) = torch.autograd.grad(y, xin, lay(dy))
+    for b in range(B):
+        a = angles64(pos[b], inv_freq)[:, None]
+        for got, src, sign in ((y, x, 1.0), (dx, dy, -1.0)):
+            src = src[b].double()
+            ref = turn64(src, a, interleaved, 1.0, sign)
+            tol = half_step(dtype) * ref.abs() + 2 ** -20 * reach(src, rot // 2, interleaved) + tiny(dtype)
+            assert ((lay(got)[b].double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("T,H,Hk,D,rot,interleaved,shared,dtype", [
+    (25603, 8, 8, 128, 128, False, False, torch.bfloat16), (25603, 12, 4, 128, 64, True, True, torch.float16),
+    (6001, 16, 16, 128, 128, False, False, torch.bfloat16), (6001, 16, 16, 128, 128, True, True, torch.bfloat16),
+    (6001, 16, 16, 128, 44, False, True, torch.float16), (6001, 16, 16, 128, 42, False, False, torch.bfloat16),
+    (8003, 12, 4, 64, 64, False, True, torch.float16), (8003, 12, 4, 64, 22, False, False, torch.bfloat16),
+    (10007, 24, 24, 16, 16, False, False, torch.bfloat16), (10007, 40, 8, 32, 24, True, True, torch.bfloat16)])
+def test_norm_rotary_of_ranges_in_several_tiles(T, H, Hk, D, rot, interleaved, shared, dtype):
+    """As above for the norms, whose backward carries the weights' gradients from tile to tile.  dw: every addition of a thread's
+    tokens, of a CTA's heads where they share a weight, and of the shares (32 groups, then those) rounds what has been added so
+    far by 2^-24; each term is off by 2^-19 of its size."""
+    from forgetting_transformer_b200 import _lib
+    B, eps = 3, 1e-5
+    assert several_tiles(2, B, T, H + Hk, D, rot, interleaved) and (T < 25603 or several_tiles(1, B, T, H + Hk, D, rot, interleaved))
+    inv_freq, _ = fox.rotary_frequencies(rot, device="cuda")
+    pos = torch.randint(0, 50000, (B, T), generator=torch.Generator().manual_seed(T)).int().cuda()
+    x = [big(T + i, B, T, h, D, dtype=dtype) for i, h in enumerate((H, Hk))]
+    dy = [big(T + 2 + i, B, T, h, D, dtype=dtype) for i, h in enumerate((H, Hk))]
+    w = [1 + 0.3 * data(T + 4 + i, D if shared else h * D, dtype=torch.float32) for i, h in enumerate((H, Hk))]
+    leaves = [t.detach().requires_grad_() for t in (*x, *w)]
+    out = fox.qk_norm_rotary(*leaves, inv_freq, pos, eps=eps, interleaved=interleaved)
+    grads = torch.autograd.grad(out, leaves, dy)
+    h16 = half_step(dtype)
+    ranges = _lib.load().fox_qk_norm_rotary_partials(B, T, H, Hk, D)
+    for i, heads in enumerate((H, Hk)):
+        w64 = w[i].double().view(-1, D)
+        dw = terms = 0
+        for b in range(B):
+            a = angles64(pos[b], inv_freq)[:, None]
+            x64, dy64 = x[i][b].double(), dy[i][b].double()
+            r = torch.rsqrt(x64.pow(2).mean(-1, keepdim=True) + eps)
+            xhat = x64 * r
+            n = xhat * w64
+            ref = turn64(n, a, interleaved)
+            assert ((out[i][b].double() - ref).abs() <= h16 * ref.abs() + 2 ** -19 * reach(n, rot // 2, interleaved) + tiny(dtype)).all()
+            dn, m = turn64(dy64, a, interleaved, 1.0, -1.0), reach(dy64, rot // 2, interleaved)
+            dx = r * (dn * w64 - xhat * (dn * w64 * xhat).mean(-1, keepdim=True))
+            size = r * (m * w64.abs() + xhat.abs() * (m * w64 * xhat).abs().mean(-1, keepdim=True))
+            assert ((grads[i][b].double() - dx).abs() <= h16 * dx.abs() + 2 ** -18 * size + tiny(dtype)).all()
+            axes = (0, 1) if shared else (0,)
+            dw, terms = dw + (dn * xhat).sum(axes).flatten(), terms + (m * xhat.abs()).sum(axes).flatten()
+        over = H + Hk if shared else 1
+        chain = -(-B * T // ranges) + over + -(-ranges // 32) * over + 32
+        assert ((grads[2 + i].double() - dw).abs() <= (2 ** -19 + chain * 2 ** -24) * terms).all()

@@ -317,3 +317,13 @@ def test_module_refuses_its_first_call_in_a_capture(monkeypatch):
         m.inv_freq(gpu)
     m._on_device[gpu] = F32
     assert m.inv_freq(gpu) is F32 and m.inv_freq(torch.device("cpu")).shape == (32,)
+
+
+def test_ranges_of_a_launch():
+    """The ranges that a backward's shares are counted by are those that its tokens are cut into."""
+    lib = _lib.load()
+    for B, T, H, Hk, D in ((3, 6001, 16, 16, 128), (3, 8003, 12, 4, 64), (1, 1, 1, 1, 16), (3, 10007, 24, 24, 16), (2, 8192, 33, 11, 128)):
+        for half, interleaved in ((D // 2, 0), (D // 2, 1), (5, 0)):
+            per = lib.fox_rotary_range(2, B, T, H + Hk, D, half, interleaved)
+            assert lib.fox_qk_norm_rotary_partials(B, T, H, Hk, D) == -(-B * T // per)
+    assert lib.fox_rotary_range(3, 1, 1, 1, 64, 32, 0) == 1 and lib.fox_rotary_range(0, 0, 1, 1, 64, 32, 0) == 1
