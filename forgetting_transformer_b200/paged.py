@@ -139,7 +139,9 @@ class PagedFgateCache:
         paged_update(*self[layer_idx], k, v, log_fgate, slots, gate_is_logit=gate_is_logit)
 
     def attend(self, layer_idx: int, q: torch.Tensor, *, sm_scale: Optional[float] = None) -> torch.Tensor:
-        """One query per request, (max_requests, heads, head_dim), against all of its tokens."""
+        """One query per request, (max_requests, heads, head_dim), against all of its tokens.  Where requests bring different numbers
+        of tokens, those of their last ones: ``q[(t.starts[1:].long() - 1).clamp(0, len(q) - 1)]`` (a request that brings none, or is
+        granted none, gets another's query there: its row of the result says nothing)."""
         return paged_forgetting_attention(q, *self[layer_idx], self.block_table, self.lengths, sm_scale=sm_scale)
 
     def crop(self, keep: torch.Tensor) -> None:

@@ -513,3 +513,63 @@ def test_generation_step_in_a_graph():
     k = torch.stack(rows).view(40, R, 3, H, D)[:, :, 1]
     for r in range(R):
         assert torch.equal(cache.history(0, r, 40)[0][0].transpose(0, 1), k[:, r])
+
+
+# ------------------------------------------------------------------ ends of ranges
+@pytest.mark.parametrize("pages,some_are_refused", [(9000, False), (3000, True)])
+def test_tables_of_more_requests_than_a_block_keeps(pages, some_are_refused):
+    """More requests than the placing kernel holds in shared memory, and more tokens than the scanning CTA places by itself."""
+    R, width, page, most, max_tokens = 5003, 4, 16, 12, 23000
+    rng = __import__("random").Random(R + pages)
+    a = Allocator(R, width, pages, page)
+    lengths, table = i32([0] * R), torch.full((R, width), -1, dtype=torch.int32, device="cuda")
+    free, num_free = i32(a.free), i32([pages])
+    refused = False
+    for step in range(6):
+        new = [rng.choice([0, 1, 1, rng.randint(0, most)]) for _ in range(R)]
+        t = fox.page_tables(lengths, i32(new), table, free, num_free, page, max_tokens, inplace=step % 2 == 1)
+        starts, granted, tokens = a.extend(new, max_tokens)
+        lengths, num_free = t.lengths, t.num_free
+        refused = refused or granted != new
+        assert t.starts.tolist() == starts and t.granted.tolist() == granted
+        assert lengths.tolist() == a.lengths and num_free.tolist() == [len(a.free)]
+        assert list(zip(t.requests.tolist(), t.positions.tolist(), t.slots.tolist())) == tokens
+        assert table.tolist() == a.table
+        if step == 3:
+            keep = [rng.choice([0, n, n // 2, n + 7, -1]) for n in a.lengths]
+            fox.release_pages(lengths, i32(keep), table, free, num_free, page)
+            a.crop(keep)
+            assert lengths.tolist() == a.lengths and table.tolist() == a.table and free[:len(a.free)].tolist() == a.free
+    assert refused == some_are_refused
+
+
+@pytest.mark.parametrize("T,H,Hk,D,page", [(18944, 2, 2, 16, 16), (19003, 6, 3, 32, 64), (19111, 5, 5, 128, 32), (25001, 24, 24, 64, 64)])
+@pytest.mark.parametrize("gates", ["log", "fp32"])
+def test_rows_of_long_prompts_into_pages(T, H, Hk, D, page, gates):
+    """Calls large enough for eight tokens ahead (16 tiles of 8 tokens to an SM), the last tile ragged."""
+    assert -(-T // 8) >= 16 * 148
+    test_rows_into_pages(T, H, Hk, D, page, gates, torch.bfloat16)
+
+
+def test_packed_batch_by_its_tables():
+    """The queries of a packed batch found on the device, by the tables' own starts: a prompt, single tokens, a place without a request, a
+    request with nothing new, and one that is refused and keeps what it has."""
+    H, Hk, D, R = 4, 2, 64, 6
+    cache = fox.PagedFgateCache(1, 20, 16, H, D, R, 200, num_kv_heads=Hk)
+
+    def step(new, room, seed):
+        t = cache.extend(i32(new), room)
+        k, v = [torch.randn(room, Hk, D, generator=gen(seed + i)).bfloat16().cuda() for i in range(2)]
+        cache.update(0, k, v, -torch.rand(room, H, generator=gen(seed + 2)).cuda(), t.slots)
+        return t
+    step([40, 0, 7, 33, 1, 5], 90, 1)
+    new = [1, 0, 60, 1, 0, 400]             # (the last is longer than its row)
+    t = step(new, 70, 5)
+    q = torch.randn(70, H, D, generator=gen(9)).bfloat16().cuda()
+    last = (t.starts[1:].long() - 1).clamp(0, q.shape[0] - 1)
+    out = cache.attend(0, q[last])
+    assert t.granted.tolist() == [1, 0, 60, 1, 0, 0] and cache.lengths.tolist() == [41, 0, 67, 34, 1, 5]
+    assert last.tolist()[:4] == [0, 0, 60, 61]
+    L = fox.paged_forgetting_attention(q[last], *cache[0], cache.block_table, cache.lengths, return_log_normalizer=True)[1]
+    check(q[last], *cache[0], cache.block_table, cache.lengths, None, (out, L))
+    assert not out[1].any()
