@@ -623,6 +623,7 @@ extern "C" int fox_qk_norm_rotary_fwd(int device, void* stream, int dtype, int64
 
 extern "C" int64_t fox_rotary_range(int kind, int64_t B, int64_t T, int64_t heads, int64_t D, int64_t half, int interleaved) {
   if (kind < kTurn || kind > kNormBack || B <= 0 || T <= 0 || heads <= 0 || (D != 16 && D != 32 && D != 64 && D != 128)) return 1;
+  if (heads > 2 * 65535 || T > kRotTokens || B > kRotTokens / T) return 1;
   return rotary_grid(static_cast<RotaryKind>(kind), kind != kNormBack && rotary_mode(half, interleaved) == kAny, heads, D, B * T).per_cta;
 }
 

@@ -327,3 +327,4 @@ def test_ranges_of_a_launch():
             per = lib.fox_rotary_range(2, B, T, H + Hk, D, half, interleaved)
             assert lib.fox_qk_norm_rotary_partials(B, T, H, Hk, D) == -(-B * T // per)
     assert lib.fox_rotary_range(3, 1, 1, 1, 64, 32, 0) == 1 and lib.fox_rotary_range(0, 0, 1, 1, 64, 32, 0) == 1
+    assert lib.fox_rotary_range(0, 2 ** 40, 2 ** 40, 1, 64, 32, 0) == 1 and lib.fox_rotary_range(0, 1, 1, 2 ** 40, 64, 32, 0) == 1
