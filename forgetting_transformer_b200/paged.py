@@ -68,7 +68,8 @@ def page_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, block_table: to
 def release_pages(lengths: torch.Tensor, keep: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                   num_free: torch.Tensor, page_size: int) -> None:
     """Cuts every request to its first ``keep`` (R,) tokens (0: ends it; more than it has: as it is); pages that are not needed
-    any more go back on the stack.  Everything in place, as ``page_tables`` takes it."""
+    any more go back on the stack.  Everything in place, as ``page_tables`` takes it.  A page that is in two tables (the attention reads
+    such tables) would go back twice: only one of them may have it when its request is cut."""
     (_host or _load_host()).release_pages(lengths, keep, block_table, free_pages, num_free, page_size)
 
 
