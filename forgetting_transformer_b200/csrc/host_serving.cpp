@@ -607,6 +607,8 @@ FOX_PY(py_paged_update) {
   {
     pybind11::gil_scoped_release no_gil;
     const Pool p = check_pool(kp, vp, gp, 1);
+    for (int i = 0; i < 2; ++i)   // (the attention may read gates that are alike for all heads)
+      check_that(gp.size(i) == 1 || gp.stride(i) > 0, "gate_pages must not be expanded where they are written: heads would overwrite one another");
     check_that(k_in.dim() == 3 && v_in.dim() == 3 && gates.dim() == 2 && slots.dim() == 1,
                "k, v must have 3 dimensions (tokens, heads, head dim), gates 2 and slots 1");
     const int64_t T = k_in.size(0);

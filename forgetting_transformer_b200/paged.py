@@ -78,9 +78,9 @@ def paged_update(k_pages: torch.Tensor, v_pages: torch.Tensor, gate_pages: torch
     """Writes keys and values (T, Hk, D) and log gates (T, H) of T tokens into their slots.
 
     k_pages, v_pages (pages, Hk, page_size, D) in fp16 / bf16, rows contiguous and 16-byte aligned; gate_pages (pages, H,
-    page_size) fp32; slots (T,) int32 / int64.  A slot outside the pool (-1) leaves its token out; of tokens with the same slot
-    any one's values may stay, piece by piece.  ``gate_is_logit``: the gates are logits (fp16 / bf16 / fp32) and their log
-    sigmoid is written.  No gradients and no tangents."""
+    page_size) fp32, not expanded; slots (T,) int32 / int64.  A slot outside the pool (-1) leaves its token out; of tokens with the
+    same slot any one's values may stay, piece by piece, and k, v may not be rows that the call writes.  ``gate_is_logit``: the
+    gates are logits (fp16 / bf16 / fp32) and their log sigmoid is written.  No gradients and no tangents."""
     (_host or _load_host()).paged_update(k_pages, v_pages, gate_pages, k, v, log_fgate, slots, gate_is_logit)
 
 

@@ -328,3 +328,14 @@ def test_ranges_of_a_launch():
             assert lib.fox_qk_norm_rotary_partials(B, T, H, Hk, D) == -(-B * T // per)
     assert lib.fox_rotary_range(3, 1, 1, 1, 64, 32, 0) == 1 and lib.fox_rotary_range(0, 0, 1, 1, 64, 32, 0) == 1
     assert lib.fox_rotary_range(0, 2 ** 40, 2 ** 40, 1, 64, 32, 0) == 1 and lib.fox_rotary_range(0, 1, 1, 2 ** 40, 64, 32, 0) == 1
+
+
+def test_expanded_gate_pages_are_not_written():
+    """Several heads' gates in one place would leave any one of them there.  Reading such pages is allowed."""
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)
+    k, v, g = pages()
+    for shared in (g[:, :1].expand(-1, 2, -1), g[:1].expand(5, -1, -1)):
+        with pytest.raises(AssertionError, match="must not be expanded"):
+            fox.paged_update(k, v, shared, bf(4, 2, 64), bf(4, 2, 64), torch.zeros(4, 2), i(4))
+        with pytest.raises(_lib.FoxError, match="no CPU path"):
+            fox.paged_forgetting_attention(bf(3, 2, 64), k, v, shared, i(3, 4), i(3))
